@@ -49,7 +49,10 @@ COMMON = [
 # no NaN operands: its running maxima then need no quieting of each operand before v_max (the
 # scores are MFMA and FMA results, never signalling NaNs), about 12 VALU instructions fewer per
 # 64-key tile. Host code keeps full NaN semantics (its argument checks test for NaN).
-DEVICE_FLAGS = {"attention_fwd.hip": ["-Xarch_device", "-fno-honor-nans"]}
+# AdamW's states are rounded operation by operation: a contracted multiply-add could move an 8-bit
+# code that lies next to a border.
+DEVICE_FLAGS = {"attention_fwd.hip": ["-Xarch_device", "-fno-honor-nans"],
+                "adamw.hip": ["-ffp-contract=off"]}
 
 
 def sources():

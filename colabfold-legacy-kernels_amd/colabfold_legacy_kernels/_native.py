@@ -83,11 +83,35 @@ PROTOTYPES = {
     "clk_triangle_multiply": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
                                       c_void_p, c_void_p, c_void_p, c_size, c_i64, c_i64, c_int,
                                       c_f32]),
+    "clk_embedding_fwd": (c_int, [c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_i64,
+                                  c_i64, c_i64, c_f32]),
+    "clk_embedding_bwd_workspace_size": (c_size, [c_i64, c_i64, c_i64]),
+    "clk_embedding_bwd": (c_int, [c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
+                                  c_size, c_i64, c_i64, c_i64, c_f32]),
+    "clk_residual_norm_fwd": (c_int, [c_void_p, c_int, c_int] + [c_void_p] * 10 +
+                              [c_i64, c_i64, c_f32]),
+    "clk_residual_norm_bwd_workspace_size": (c_size, [c_i64, c_i64]),
+    "clk_residual_norm_bwd": (c_int, [c_void_p, c_int, c_int] + [c_void_p] * 18 +
+                              [c_size, c_i64, c_i64, c_f32]),
+    "clk_adamw_table": (c_int, [c_void_p, c_i64, c_int, c_void_p, c_size,
+                                ctypes.POINTER(c_i64)]),
+    "clk_adamw_step": (c_int, [c_void_p, c_void_p, c_i64, c_int, c_i64] + [ctypes.c_double] * 6 +
+                       [c_void_p]),
+    "clk_adamw_states": (c_int, [c_void_p, c_void_p, c_i64, c_int, c_void_p, c_void_p]),
 }
+
+
+class AdamwTensor(ctypes.Structure):
+    """clk_adamw_tensor."""
+    _fields_ = [("param", c_void_p), ("grad", c_void_p), ("exp_avg", c_void_p),
+                ("exp_avg_sq", c_void_p), ("scales", c_void_p), ("copy", c_void_p),
+                ("numel", c_i64), ("grad_dtype", c_int), ("copy_dtype", c_int)]
 
 # Status codes (clk_status) and dtype codes (clk_dtype).
 OK, INVALID_ARGUMENT, UNIMPLEMENTED, INTERNAL = 0, 3, 12, 13
-U8, F16, F32, BF16 = 6, 10, 11, 16
+S32, S64, U8, F16, F32, BF16 = 4, 5, 6, 10, 11, 16
+# Norms (clk_norm).
+NORM_LAYER, NORM_RMS = 0, 1
 
 
 def load(path=None):

@@ -9,8 +9,10 @@ buffers:
   gated_dual_proj(x, wp, bp, wg, bg, mask)                   VoltaGdp   (cuda/volta_ops.cu:254-265)
 
 and the targets the reference lacks: attention_fwd (also returns the logsumexp), attention_bwd,
-layer_norm_bwd and ln_gated_dual_proj. An invalid call raises InvalidArgument (a ValueError), as
-the reference handlers return ffi::Error::InvalidArgument; a launch failure raises InternalError.
+layer_norm_bwd and ln_gated_dual_proj, and what closes a training step around the blocks: embedding
+and embedding_bwd, residual_norm and residual_norm_bwd, AdamWPlan and adamw_step. An invalid call
+raises InvalidArgument (a ValueError), as the reference handlers return
+ffi::Error::InvalidArgument; a launch failure raises InternalError.
 
 Torch is used only for device memory and the current stream; all arithmetic runs in the HIP
 library, and a missing library raises FileNotFoundError (there is no fallback path).
@@ -29,7 +31,10 @@ __all__ = [
     "attention_gate", "attention_gate_bwd", "attention_gated", "attention_gated_fwd",
     "layer_norm", "layer_norm_bwd",
     "gated_dual_proj", "ln_gated_dual_proj",
+    "embedding", "embedding_bwd", "residual_norm", "residual_norm_bwd",
+    "AdamWPlan", "adamw_zero_states", "adamw_step", "adamw_hyper", "adamw_states",
     "AttentionFunction", "GatedAttentionFunction", "LayerNormFunction",
+    "EmbeddingFunction", "ResidualNormFunction",
 ]
 
 
@@ -566,6 +571,264 @@ def triangle_multiply(z, mask, ln_in, weights, biases, ln_center, outgoing=True,
     return out
 
 
+_ID_DTYPES = {torch.int32: _native.S32, torch.int64: _native.S64}
+
+
+def _id_code(ids, what):
+    code = _ID_DTYPES.get(ids.dtype)
+    if code is None:
+        _fail(what, "ids must be int32 or int64, got %s" % ids.dtype)
+    return code
+
+
+def embedding(table, ids, scale=1.0):
+    """scale * table[ids] for table [V,C] (f16, bf16 or f32) and ids (int32 or int64) of any shape:
+    [..., C]. An id outside [0, V) is an absent token: its row is zero."""
+    what = "embedding"
+    index = _require([("table", table), ("ids", ids)], what)
+    _shape_check(table.dim() == 2, what, "table must be [V,C]")
+    v, c = table.shape
+    code, id_code = _dtype_code(table, (_native.F16, _native.BF16, _native.F32), what), _id_code(
+        ids, what)
+    out = table.new_empty(tuple(ids.shape) + (c,))
+    _launch(index, _native.lib().clk_embedding_fwd, code, table.data_ptr(), id_code,
+            ids.data_ptr(), out.data_ptr(), ids.numel(), v, c, float(scale))
+    return out
+
+
+def embedding_bwd(dout, ids, rows, scale=1.0):
+    """The gradient of embedding's table: float32 [rows,C], scale times the sum of dout [..., C]
+    over the tokens of each row, in a fixed order; zero for rows that no token names."""
+    what = "embedding_bwd"
+    index = _require([("dout", dout), ("ids", ids)], what)
+    _shape_check(dout.dim() >= 1 and dout.shape[:-1] == ids.shape, what,
+                 "dout must be ids' shape and [C]")
+    c, rows = dout.shape[-1], int(rows)
+    _shape_check(rows >= 0, what, "rows must not be negative")
+    code, id_code = _dtype_code(dout, (_native.F16, _native.BF16, _native.F32), what), _id_code(
+        ids, what)
+    lib = _native.lib()
+    m = ids.numel()
+    wsb = lib.clk_embedding_bwd_workspace_size(m, rows, c)
+    ws = _workspace(dout, wsb)
+    dtable = dout.new_empty((rows, c), dtype=torch.float32)
+    _launch(index, lib.clk_embedding_bwd, code, dout.data_ptr(), id_code, ids.data_ptr(),
+            dtable.data_ptr(), ws.data_ptr(), wsb, m, rows, c, float(scale))
+    return dtable
+
+
+_NORMS = {"layer": _native.NORM_LAYER, "rms": _native.NORM_RMS}
+
+
+def _norm_pair(pair, c, name, what):
+    """(scale, offset) of a norm: float32 [C] each, the offset or the whole pair may be None."""
+    if pair is None:
+        return None, None
+    scale, offset = pair
+    _shape_check(scale is not None, what, "%s needs a scale" % name)
+    for t in (scale, offset):
+        if t is not None and (t.shape != (c,) or t.dtype != torch.float32):
+            _fail(what, "%s must be float32 [C]" % name)
+    return scale, offset
+
+
+def _residual_args(rows, vectors, kind, what):
+    """(device, dtype code, norm code, M, C) of the [..., C] operands `rows`, all alike."""
+    index = _require(rows + vectors, what)
+    if kind not in _NORMS:
+        _fail(what, "kind must be 'layer' or 'rms', got %r" % (kind,))
+    first = rows[0][1]
+    _shape_check(first.dim() >= 1, what, "%s must have at least one axis" % rows[0][0])
+    for name, t in rows:
+        if t is not None and (t.shape != first.shape or t.dtype != first.dtype):
+            _fail(what, "%s must match %s" % (name, rows[0][0]))
+    code = _dtype_code(first, (_native.F16, _native.BF16, _native.F32), what)
+    c = first.shape[-1]
+    return index, code, _NORMS[kind], first.numel() // c if c else 0, c
+
+
+def residual_norm(x, o, gate=None, post=None, res_scale=None, pre=None, kind="layer", eps=1e-5):
+    """(r, h): r = x + res_scale * sigmoid(gate) * N_post(o), a block's output o joined with the
+    residual stream x, and h = N_pre(r), the next block's input (None without pre). x, o, gate
+    [..., C] of one dtype (f16, bf16, f32); post and pre: (scale, offset) float32 [C] of a LayerNorm
+    or, with kind "rms", of an RMS norm, the offset None where there is none; res_scale float32 [C].
+    gate, post, res_scale and pre may each be None: no gate, no norm, 1, no norm."""
+    what = "residual_norm"
+    c = x.shape[-1] if isinstance(x, torch.Tensor) and x.dim() else 0
+    post_scale, post_offset = _norm_pair(post, c, "post", what)
+    pre_scale, pre_offset = _norm_pair(pre, c, "pre", what)
+    index, code, norm, m, c = _residual_args(
+        [("x", x), ("o", o), ("gate", gate)],
+        [("post", post_scale), ("post", post_offset), ("res_scale", res_scale),
+         ("pre", pre_scale), ("pre", pre_offset)], kind, what)
+    if res_scale is not None:
+        _shape_check(res_scale.shape == (c,) and res_scale.dtype == torch.float32, what,
+                     "res_scale must be float32 [C]")
+    r = torch.empty_like(x)
+    h = torch.empty_like(x) if pre_scale is not None else None
+    _launch(index, _native.lib().clk_residual_norm_fwd, code, norm, x.data_ptr(), o.data_ptr(),
+            _ptr(gate), _ptr(post_scale), _ptr(post_offset), _ptr(res_scale), _ptr(pre_scale),
+            _ptr(pre_offset), r.data_ptr(), _ptr(h), m, c, float(eps))
+    return r, h
+
+
+def residual_norm_bwd(r, o, gate, post, res_scale, pre, dr, dh, kind="layer", eps=1e-5):
+    """Gradients of residual_norm from its result r and the gradients dr of r and dh of h (dr may
+    be None: zero; dh is given with pre, and only with it): (dx, do, dgate, dpost_scale,
+    dpost_offset, dres_scale, dpre_scale, dpre_offset), the first three in r's dtype, the others
+    float32 [C], None for what was not given."""
+    what = "residual_norm_bwd"
+    c = r.shape[-1] if isinstance(r, torch.Tensor) and r.dim() else 0
+    post_scale, post_offset = _norm_pair(post, c, "post", what)
+    pre_scale, pre_offset = _norm_pair(pre, c, "pre", what)
+    index, code, norm, m, c = _residual_args(
+        [("r", r), ("o", o), ("gate", gate), ("dr", dr), ("dh", dh)],
+        [("post", post_scale), ("post", post_offset), ("res_scale", res_scale),
+         ("pre", pre_scale), ("pre", pre_offset)], kind, what)
+    if res_scale is not None:
+        _shape_check(res_scale.shape == (c,) and res_scale.dtype == torch.float32, what,
+                     "res_scale must be float32 [C]")
+    _shape_check((dh is not None) == (pre_scale is not None), what,
+                 "dh is given with pre, and only with it")
+    _shape_check(dr is not None or dh is not None, what, "dr or dh must be given")
+    lib = _native.lib()
+    wsb = lib.clk_residual_norm_bwd_workspace_size(m, c)
+    ws = _workspace(r, wsb)
+    dx, do = torch.empty_like(r), torch.empty_like(r)
+    dgate = torch.empty_like(r) if gate is not None else None
+    # The five column sums share one allocation; each begins at a multiple of 16 bytes.
+    c4 = -(-c // 4) * 4
+    sums = r.new_empty((5, c4), dtype=torch.float32)
+    dpost_scale, dpost_offset, dres, dpre_scale, dpre_offset = (
+        sums[i, :c] if t is not None else None
+        for i, t in enumerate((post_scale, post_offset, res_scale, pre_scale, pre_offset)))
+    _launch(index, lib.clk_residual_norm_bwd, code, norm, r.data_ptr(), o.data_ptr(), _ptr(gate),
+            _ptr(post_scale), _ptr(post_offset), _ptr(res_scale), _ptr(pre_scale), _ptr(dr),
+            _ptr(dh), dx.data_ptr(), do.data_ptr(), _ptr(dgate), _ptr(dpost_scale),
+            _ptr(dpost_offset), _ptr(dres), _ptr(dpre_scale), _ptr(dpre_offset), ws.data_ptr(),
+            wsb, m, c, float(eps))
+    return dx, do, dgate, dpost_scale, dpost_offset, dres, dpre_scale, dpre_offset
+
+
+_STATE_BLOCK = 256  # elements that share the two scales of 8-bit states
+
+
+def adamw_zero_states(params, state_bits=32):
+    """Zero states for AdamWPlan: (exp_avgs, exp_avg_sqs, scales), float32 tensors and None with 32
+    bits; int8, uint8 and float32 [ceil(numel/256), 2] tensors with 8."""
+    if state_bits == 32:
+        return ([torch.zeros_like(p, dtype=torch.float32) for p in params],
+                [torch.zeros_like(p, dtype=torch.float32) for p in params], None)
+    if state_bits != 8:
+        _fail("adamw_zero_states", "state_bits must be 8 or 32")
+    return ([torch.zeros_like(p, dtype=torch.int8) for p in params],
+            [torch.zeros_like(p, dtype=torch.uint8) for p in params],
+            [p.new_zeros((-(-p.numel() // _STATE_BLOCK), 2), dtype=torch.float32)
+             for p in params])
+
+
+class AdamWPlan:
+    """The tensors of AdamW steps, checked and listed once. params: float32 master weights; grads:
+    their gradients (f32, bf16 or f16), which every step reads; exp_avgs, exp_avg_sqs: the states,
+    float32, or int8 and uint8 codes with scales float32 [ceil(numel/256), 2] (adamw_zero_states
+    makes either); copies: the bf16 or f16 working copies that a step also writes (or None, as a
+    whole or for single tensors). All contiguous and on one device; nothing that a step writes may
+    overlap anything else. The plan keeps the tensors' storages as they were when it was made: a
+    tensor whose storage is replaced or resized needs a new plan. ``numel`` and ``starts`` are the
+    tensors' sizes and their places in the buffers of adamw_states."""
+
+    def __init__(self, params, grads, exp_avgs, exp_avg_sqs, scales=None, copies=None):
+        what = "AdamWPlan"
+        params, grads = list(params), list(grads)
+        exp_avgs, exp_avg_sqs = list(exp_avgs), list(exp_avg_sqs)
+        n = len(params)
+        scales = [None] * n if scales is None else list(scales)
+        copies = [None] * n if copies is None else list(copies)
+        lists = (params, grads, exp_avgs, exp_avg_sqs, scales, copies)
+        names = ("params", "grads", "exp_avgs", "exp_avg_sqs", "scales", "copies")
+        _shape_check(n > 0, what, "at least one tensor")
+        for name, ts in zip(names, lists):
+            _shape_check(len(ts) == n, what, "%s must have as many tensors as params" % name)
+            for t in ts:
+                if t is None and name not in ("scales", "copies"):
+                    _fail(what, "%s must be tensors" % name)
+        self.device_index = _require([(name, t) for name, ts in zip(names, lists) for t in ts],
+                                     what)
+        self.state_bits = 8 if exp_avgs[0].dtype == torch.int8 else 32
+        kinds = (torch.int8, torch.uint8) if self.state_bits == 8 else (torch.float32,) * 2
+        table = (_native.AdamwTensor * n)()
+        self.numel, self.starts, self.size = [], [], 0
+        for i, (p, g, m, v, s, c) in enumerate(zip(*lists)):
+            size = p.numel()
+            _shape_check(p.dtype == torch.float32, what, "params must be float32")
+            for name, t in (("grads", g), ("exp_avgs", m), ("exp_avg_sqs", v), ("copies", c)):
+                if t is not None and t.shape != p.shape:
+                    _fail(what, "%s must have the shapes of params" % name)
+            if m.dtype != kinds[0] or v.dtype != kinds[1]:
+                _fail(what, "states must all be float32, or all int8 and uint8")
+            if self.state_bits == 8:
+                if s is None or s.dtype != torch.float32 or s.shape != (
+                        -(-size // _STATE_BLOCK), 2):
+                    _fail(what, "scales must be float32 [ceil(numel/256), 2]")
+            elif s is not None:
+                _fail(what, "32-bit states have no scales")
+            grad_code = _dtype_code(g, (_native.F16, _native.BF16, _native.F32), what)
+            copy_code = 0 if c is None else _dtype_code(c, (_native.F16, _native.BF16), what)
+            table[i] = _native.AdamwTensor(p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(),
+                                           _ptr(s), _ptr(c), size, grad_code, copy_code)
+            self.numel.append(size)
+            self.starts.append(self.size)
+            self.size += -(-size // _STATE_BLOCK) * _STATE_BLOCK
+        self._tensors = lists
+        # Autograd's count of in-place changes, for a graph that saved a weight or its copy.
+        self._changed = [t for t in params + copies if t is not None and not t.is_inference()]
+        lib, chunks = _native.lib(), ctypes.c_int64(0)
+        _check(lib.clk_adamw_table(table, n, self.state_bits, None, 0, ctypes.byref(chunks)))
+        self.chunks = chunks.value
+        host = torch.empty(max(64 * self.chunks, 64), dtype=torch.uint8)
+        _check(lib.clk_adamw_table(table, n, self.state_bits, host.data_ptr(), host.numel(),
+                                   ctypes.byref(chunks)))
+        # A copy from pageable memory has ended when the call returns: any stream may use it.
+        self._table = host.to(params[0].device)
+
+
+def adamw_step(plan, step, lr, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.0, grad_scale=1.0,
+               hyper=None):
+    """One AdamW step over the tensors of a plan, in place; step counts from 1. With hyper (float32
+    [4] on the plan's device, as adamw_hyper gives it) the kernel reads lr, the bias corrections and
+    grad_scale from there when it runs, and step, lr and grad_scale are not looked at: a captured
+    graph can be replayed with other values."""
+    what = "adamw_step"
+    if hyper is not None:
+        index = _require([("hyper", hyper)], what)
+        _shape_check(index == plan.device_index and hyper.shape == (4,) and
+                     hyper.dtype == torch.float32, what,
+                     "hyper must be float32 [4] on the plan's device")
+        step, lr, grad_scale = 1, 0.0, 1.0
+    _launch(plan.device_index, _native.lib().clk_adamw_step, plan._table.data_ptr(), plan.chunks,
+            plan.state_bits, int(step), float(lr), float(beta1), float(beta2), float(eps),
+            float(weight_decay), float(grad_scale), _ptr(hyper))
+    torch.autograd.graph.increment_version(plan._changed)
+
+
+def adamw_hyper(step, lr, beta1=0.9, beta2=0.999, grad_scale=1.0):
+    """The values of adamw_step's hyper for a step, float32 [4] on the host (copy them into the
+    device tensor that the graph was captured with)."""
+    return torch.tensor([lr, 1.0 - beta1 ** step, 1.0 - beta2 ** step, grad_scale],
+                        dtype=torch.float32)
+
+
+def adamw_states(plan):
+    """(exp_avg, exp_avg_sq): the plan's states as float32 (8-bit ones decoded), each in one flat
+    buffer in which tensor i is [plan.starts[i] : plan.starts[i] + plan.numel[i]]."""
+    device = plan._table.device
+    m = torch.empty(plan.size, dtype=torch.float32, device=device)
+    v = torch.empty_like(m)
+    _launch(plan.device_index, _native.lib().clk_adamw_states, plan._table.data_ptr(), plan.chunks,
+            plan.state_bits, m.data_ptr(), v.data_ptr())
+    return m, v
+
+
 class AttentionFunction(torch.autograd.Function):
     """Differentiable attention: forward saves (out, lse); backward calls attention_bwd."""
 
@@ -625,3 +888,51 @@ class LayerNormFunction(torch.autograd.Function):
         x, scale = ctx.saved_tensors
         dx, dscale, doffset = layer_norm_bwd(x, scale, dy.contiguous(), ctx.eps)
         return dx, dscale, doffset, None
+
+
+class EmbeddingFunction(torch.autograd.Function):
+    """Differentiable embedding(table, ids, scale); the gradient of the table is summed in float32
+    and rounded to the table's dtype once."""
+
+    @staticmethod
+    def forward(ctx, table, ids, scale=1.0):
+        ctx.save_for_backward(ids)
+        ctx.scale, ctx.rows, ctx.dtype = scale, table.shape[0], table.dtype
+        return embedding(table, ids, scale)
+
+    @staticmethod
+    def backward(ctx, dout):
+        ids, = ctx.saved_tensors
+        dtable = embedding_bwd(dout.contiguous(), ids, ctx.rows, ctx.scale)
+        return dtable.to(ctx.dtype), None, None
+
+
+class ResidualNormFunction(torch.autograd.Function):
+    """Differentiable residual_norm: (r, h) of x, o, gate, post_scale, post_offset, res_scale,
+    pre_scale, pre_offset (None for what is not there), kind and eps; the backward reads r, o and
+    the gate and recomputes the statistics."""
+
+    @staticmethod
+    def forward(ctx, x, o, gate, post_scale, post_offset, res_scale, pre_scale, pre_offset,
+                kind="layer", eps=1e-5):
+        post = None if post_scale is None else (post_scale, post_offset)
+        pre = None if pre_scale is None else (pre_scale, pre_offset)
+        r, h = residual_norm(x, o, gate, post, res_scale, pre, kind, eps)
+        ctx.save_for_backward(r, o, gate, post_scale, post_offset, res_scale, pre_scale,
+                              pre_offset)
+        ctx.kind, ctx.eps = kind, eps
+        ctx.set_materialize_grads(False)
+        return r, h
+
+    @staticmethod
+    def backward(ctx, dr, dh):
+        r, o, gate, post_scale, post_offset, res_scale, pre_scale, pre_offset = ctx.saved_tensors
+        if dr is None and dh is None:
+            return (None,) * 10
+        post = None if post_scale is None else (post_scale, post_offset)
+        # Without a gradient of h the norm before the next block takes no part.
+        pre = None if dh is None else (pre_scale, pre_offset)
+        grads = residual_norm_bwd(r, o, gate, post, res_scale, pre,
+                                  None if dr is None else dr.contiguous(),
+                                  None if dh is None else dh.contiguous(), ctx.kind, ctx.eps)
+        return grads + (None, None)

@@ -1,0 +1,665 @@
+// Token embedding for gfx950: rows of a table, scaled, and the table's gradient.
+//
+//   out[i]    = scale * table[ids[i]]                       ids in [0, V); any other id is an
+//   dtable[v] = scale * sum of dout[i] over ids[i] = v      absent token: a zero row, no gradient
+//
+// The forward is one pass that writes M*C*b bytes (the rows of a table that is used often stay in
+// the L2s). The gradient sorts the tokens by row (stably, so that the order of every sum is fixed),
+// sums runs of equal rows over the sorted order and joins the runs that were cut; it reads dout
+// once, in whole rows of at least 256 bytes where a row has them, and writes the table once.
+#include "rows.hpp"
+
+namespace clk {
+namespace {
+
+constexpr int kThreads = 256;
+// ---------------------------------------------------------------------------------------------
+// Forward: a block takes `rows` whole rows; thread t takes vectors t, t + 256, ... of them, four
+// in flight, so that every wave writes consecutive vectors whatever C is.
+// ---------------------------------------------------------------------------------------------
+template <typename TR, typename ID, bool WHOLE>
+__global__ __launch_bounds__(kThreads) void embed_kernel(
+    const typename TR::elem* __restrict__ table, const ID* __restrict__ ids,
+    typename TR::elem* __restrict__ out, int64_t M, int64_t V, int C, int rows, FastDiv nvec,
+    float scale) {
+    constexpr int N = Vec<TR>::N, U = 4;
+    for (int64_t row0 = (int64_t)blockIdx.x * rows; row0 < M; row0 += (int64_t)gridDim.x * rows) {
+        const int here = (int)(M - row0 < rows ? M - row0 : rows);
+        const uint32_t total = (uint32_t)here * nvec.d;
+        for (uint32_t f0 = threadIdx.x; f0 < total; f0 += U * kThreads) {
+            int64_t id[U];
+            uint32_t r[U];
+            int col[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const uint32_t f = f0 + u * kThreads < total ? f0 + u * kThreads : f0;
+                r[u] = div_by(f, nvec);
+                col[u] = (int)(f - r[u] * nvec.d) * N;
+                id[u] = (int64_t)ids[row0 + r[u]];
+            }
+            u32x4 raw[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                raw[u] = id[u] >= 0 && id[u] < V
+                             ? load_vec<TR, WHOLE>(table + (size_t)id[u] * C, col[u], C)
+                             : u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (f0 + u * kThreads >= total) break;
+                // Absent rows are +0 whatever the scale is (a zero times infinity is NaN).
+                if (id[u] >= 0 && id[u] < V) {
+                    float v[N];
+                    unpack_vec<TR>(raw[u], v);
+#pragma unroll
+                    for (int i = 0; i < N; ++i) v[i] *= scale;
+                    raw[u] = pack_vec<TR>(v);
+                }
+                store_vec<TR, WHOLE>(out + (size_t)(row0 + r[u]) * C, col[u], C, raw[u]);
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Sorting the tokens: keys are rows of the table, V for an absent token (they come last).
+// ---------------------------------------------------------------------------------------------
+template <typename ID>
+__device__ __forceinline__ uint32_t token_key(const ID* ids, int64_t i, uint32_t V) {
+    const int64_t id = (int64_t)ids[i];
+    return id >= 0 && id < (int64_t)V ? (uint32_t)id : V;
+}
+
+// Few tokens: each one's place is the number of tokens before it, counted over all of them. M^2
+// comparisons over the whole chip, in one launch: 16 tokens a block, 16 threads a token.
+constexpr int kRankMax = 8192;  // 32 KB of keys in LDS
+constexpr int kRankTokens = 16, kRankSlices = kThreads / kRankTokens;
+template <typename ID>
+__global__ __launch_bounds__(kThreads) void embed_rank_kernel(const ID* __restrict__ ids, int M,
+                                                              uint32_t V,
+                                                              uint32_t* __restrict__ keys,
+                                                              uint32_t* __restrict__ order) {
+    __shared__ __attribute__((aligned(16))) uint32_t k[kRankMax];
+    const int padded = (M + 3) & ~3;
+    for (int i = threadIdx.x; i < padded; i += kThreads)
+        k[i] = i < M ? token_key(ids, i, V) : ~0u;  // past every token
+    __syncthreads();
+    const int slice = threadIdx.x % kRankSlices;
+    const int i = blockIdx.x * kRankTokens + threadIdx.x / kRankSlices;
+    const uint32_t mine = i < M ? k[i] : 0;
+    int before = 0;
+    for (int j = 4 * slice; j < padded; j += 4 * kRankSlices) {
+        const u32x4 o = *reinterpret_cast<const u32x4*>(k + j);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) before += o[t] < mine + (j + t < i ? 1u : 0u);
+    }
+#pragma unroll
+    for (int s = kRankSlices / 2; s > 0; s >>= 1) before += __shfl_xor(before, s);
+    if (slice == 0 && i < M) {
+        keys[before] = mine;
+        order[before] = (uint32_t)i;
+    }
+}
+
+// More tokens: a stable least-significant-digit radix sort, 8 bits a pass. A tile is 2048 tokens;
+// counts[digit][tile] is summed over the tiles of each digit (one block a digit), and the scatter
+// adds the digits before.
+constexpr int kTile = 2048, kDigits = 256;
+
+template <typename ID>
+struct FirstKeys {  // the first pass reads the ids themselves
+    const ID* ids;
+    uint32_t V;
+    __device__ __forceinline__ uint32_t key(int64_t i) const { return token_key(ids, i, V); }
+    __device__ __forceinline__ uint32_t value(int64_t i) const { return (uint32_t)i; }
+};
+struct NextKeys {
+    const uint32_t *keys, *order;
+    __device__ __forceinline__ uint32_t key(int64_t i) const { return keys[i]; }
+    __device__ __forceinline__ uint32_t value(int64_t i) const { return order[i]; }
+};
+
+template <typename SRC>
+__global__ __launch_bounds__(kThreads) void embed_count_kernel(SRC src, int64_t M, int shift,
+                                                               int64_t tiles,
+                                                               uint32_t* __restrict__ counts) {
+    __shared__ uint32_t n[kDigits];
+    n[threadIdx.x] = 0;
+    __syncthreads();
+    const int64_t base = (int64_t)blockIdx.x * kTile;
+#pragma unroll
+    for (int u = 0; u < kTile / kThreads; ++u) {
+        const int64_t i = base + u * kThreads + threadIdx.x;
+        if (i < M) atomicAdd(&n[(src.key(i) >> shift) & 255u], 1u);  // whole numbers: any order
+    }
+    __syncthreads();
+    counts[(size_t)threadIdx.x * tiles + blockIdx.x] = n[threadIdx.x];
+}
+
+// Exclusive sums of one digit's counts over the tiles, in place, and its total.
+__global__ __launch_bounds__(kThreads) void embed_scan_kernel(uint32_t* __restrict__ counts,
+                                                              int64_t tiles,
+                                                              uint32_t* __restrict__ totals) {
+    __shared__ uint32_t wave_sum[kThreads / 64];
+    uint32_t* row = counts + (size_t)blockIdx.x * tiles;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t carry = 0;
+    for (int64_t t0 = 0; t0 < tiles; t0 += kThreads) {
+        const int64_t t = t0 + threadIdx.x;
+        const uint32_t own = t < tiles ? row[t] : 0;
+        uint32_t sum = own;
+#pragma unroll
+        for (int s = 1; s < 64; s <<= 1) {
+            const uint32_t o = __shfl_up(sum, s);
+            if (lane >= s) sum += o;
+        }
+        if (lane == 63) wave_sum[wave] = sum;
+        __syncthreads();
+        uint32_t before = carry, all = 0;
+#pragma unroll
+        for (int w = 0; w < kThreads / 64; ++w) {
+            if (w < wave) before += wave_sum[w];
+            all += wave_sum[w];
+        }
+        if (t < tiles) row[t] = before + sum - own;
+        carry += all;
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) totals[blockIdx.x] = carry;
+}
+
+// Moves a tile's tokens to their places. Wave w takes the tile's w-th quarter, 64 consecutive
+// tokens a round; lanes with equal digits find each other by eight ballots, so a token's rank
+// follows the order of the tokens.
+template <typename SRC>
+__global__ __launch_bounds__(kThreads) void embed_scatter_kernel(
+    SRC src, int64_t M, int shift, int64_t tiles, const uint32_t* __restrict__ counts,
+    const uint32_t* __restrict__ totals, uint32_t* __restrict__ keys,
+    uint32_t* __restrict__ order) {
+    constexpr int kWaves = kThreads / 64, kRounds = kTile / kThreads;
+    __shared__ uint32_t n[kWaves][kDigits];
+    __shared__ uint32_t wave_sum[kWaves];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) n[w][threadIdx.x] = 0;
+    // Exclusive sum of the digits' totals (one thread a digit).
+    const uint32_t own = totals[threadIdx.x];
+    uint32_t sum = own;
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) {
+        const uint32_t o = __shfl_up(sum, s);
+        if (lane >= s) sum += o;
+    }
+    if (lane == 63) wave_sum[wave] = sum;
+    __syncthreads();
+    uint32_t first = sum - own;
+    for (int w = 0; w < wave; ++w) first += wave_sum[w];
+    first += counts[(size_t)threadIdx.x * tiles + blockIdx.x];
+
+    const int64_t base = (int64_t)blockIdx.x * kTile + wave * (kTile / kWaves);
+    uint32_t key[kRounds], rank[kRounds];
+#pragma unroll
+    for (int u = 0; u < kRounds; ++u) {
+        const int64_t i = base + u * 64 + lane;
+        key[u] = i < M ? src.key(i) : 0;
+    }
+#pragma unroll
+    for (int u = 0; u < kRounds; ++u) {
+        const bool there = base + u * 64 + lane < M;
+        const uint32_t digit = (key[u] >> shift) & 255u;
+        uint64_t same = __ballot(there);
+#pragma unroll
+        for (int b = 0; b < 8; ++b) {
+            const uint64_t set = __ballot((digit >> b) & 1u);
+            same &= (digit >> b) & 1u ? set : ~set;
+        }
+        const uint64_t below = same & ((1ull << lane) - 1ull);
+        if (there) {
+            // LDS operations of a wave are in order: all its lanes read before the first lane of
+            // each digit writes the new count.
+            const uint32_t had = n[wave][digit];
+            rank[u] = had + (uint32_t)__popcll(below);
+            __builtin_amdgcn_wave_barrier();
+            if (below == 0) n[wave][digit] = had + (uint32_t)__popcll(same);
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+    __syncthreads();
+    // Where each wave's tokens of a digit begin.
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        const uint32_t had = n[w][threadIdx.x];
+        n[w][threadIdx.x] = first;
+        first += had;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kRounds; ++u) {
+        const int64_t i = base + u * 64 + lane;
+        if (i < M) {
+            const uint32_t to = n[wave][(key[u] >> shift) & 255u] + rank[u];
+            keys[to] = key[u];
+            order[to] = src.value(i);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Sums of the sorted tokens. The sorted order is cut into chunks of kChunk tokens. A group of
+// LPR lanes takes one chunk and one slice of LPR vectors of the columns, keeps the running sum in
+// registers and stores it where the row ends: into the table if the run also began in the chunk,
+// else into a partial of the chunk: `tail` for a run that begins here and goes on, `head` for one
+// that began before (whether or not it goes on).
+// ---------------------------------------------------------------------------------------------
+constexpr int kChunk = 32;
+
+// First position of the sorted keys that is not below `key`.
+__device__ __forceinline__ uint32_t lower_bound(const uint32_t* keys, uint32_t M, uint32_t key) {
+    uint32_t lo = 0, n = M;
+    while (n > 0) {
+        const uint32_t half = n / 2;
+        if (keys[lo + half] < key) {
+            lo += half + 1;
+            n -= half + 1;
+        } else {
+            n = half;
+        }
+    }
+    return lo;
+}
+
+// Blocks [0, sum_blocks) sum; the others write starts[v] = first sorted token of row v, v <= V.
+template <typename TR, int LPR, bool WHOLE>
+__global__ __launch_bounds__(kThreads) void embed_sum_kernel(
+    const typename TR::elem* __restrict__ dout, const uint32_t* __restrict__ keys,
+    const uint32_t* __restrict__ order, float* __restrict__ dtable, float* __restrict__ head,
+    float* __restrict__ tail, uint32_t* __restrict__ starts, uint32_t M, uint32_t V, int C,
+    uint32_t chunks, FastDiv slices, uint32_t sum_blocks, float scale) {
+    constexpr int N = Vec<TR>::N, U = 8;
+    static_assert(kChunk % U == 0);
+    if (blockIdx.x >= sum_blocks) {
+        const uint32_t v = (blockIdx.x - sum_blocks) * kThreads + threadIdx.x;
+        if (v <= V) starts[v] = lower_bound(keys, M, v);
+        return;
+    }
+    const uint32_t group = blockIdx.x * (kThreads / LPR) + threadIdx.x / LPR;
+    const uint32_t chunk = div_by(group, slices), slice = group - chunk * slices.d;
+    if (chunk >= chunks) return;
+    const int col = (int)(slice * LPR + threadIdx.x % LPR) * N;
+    if (col >= C) return;
+    const uint32_t beg = chunk * kChunk, end = M - beg < kChunk ? M : beg + kChunk;
+    uint32_t cur = keys[beg];
+    bool began = beg == 0 || keys[beg - 1] != cur;  // the current run began in this chunk
+    float acc[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] = 0.f;
+    for (uint32_t i0 = beg; i0 < end && cur < V; i0 += U) {
+        uint32_t k[U], at[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            k[u] = i0 + u < end ? keys[i0 + u] : V;
+            at[u] = i0 + u < end ? order[i0 + u] : 0;
+        }
+        u32x4 raw[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            raw[u] = k[u] < V ? load_vec<TR, WHOLE>(dout + (size_t)at[u] * C, col, C)
+                              : u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (i0 + u >= end) break;
+            if (k[u] != cur) {
+                if (began) {
+#pragma unroll
+                    for (int i = 0; i < N; ++i) acc[i] *= scale;
+                    store_floats(dtable + (size_t)cur * C, col, C, acc);
+                } else {
+                    store_floats(head + (size_t)chunk * C, col, C, acc);
+                }
+#pragma unroll
+                for (int i = 0; i < N; ++i) acc[i] = 0.f;
+                cur = k[u];
+                began = true;
+                if (cur >= V) break;
+            }
+            float v[N];
+            unpack_vec<TR>(raw[u], v);
+#pragma unroll
+            for (int i = 0; i < N; ++i) acc[i] += v[i];
+        }
+    }
+    if (cur >= V) return;
+    if (!began) {
+        store_floats(head + (size_t)chunk * C, col, C, acc);
+    } else if (end < M && keys[end] == cur) {
+        store_floats(tail + (size_t)chunk * C, col, C, acc);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] *= scale;
+        store_floats(dtable + (size_t)cur * C, col, C, acc);
+    }
+}
+
+// Runs cut by chunk ends: tail of their first chunk plus the heads of the others. A run over at
+// most kLongRun chunks is joined by one wave, with the rows that no token named set to zero; a
+// longer one by a block of its own.
+constexpr int kLongRun = 64;
+struct Run {
+    uint32_t first, last;  // chunks
+    bool none;
+};
+__device__ __forceinline__ Run run_of(const uint32_t* starts, uint32_t v) {
+    const uint32_t s = starts[v], e = starts[v + 1];
+    return Run{s / kChunk, (e - 1) / kChunk, s == e};
+}
+
+__device__ __forceinline__ f32x4 load4(const float* p, int col, int C) {
+    float v[4];
+    load_floats<4, false>(p, col, C, 0.f, v);
+    return f32x4{v[0], v[1], v[2], v[3]};
+}
+
+__global__ __launch_bounds__(kThreads) void embed_join_kernel(
+    const float* __restrict__ head, const float* __restrict__ tail,
+    const uint32_t* __restrict__ starts, float* __restrict__ dtable, uint32_t V, int C,
+    FastDiv slices, float scale) {
+    const uint32_t items = V * slices.d, step = gridDim.x * (kThreads / 64);
+    for (uint32_t item = blockIdx.x * (kThreads / 64) + threadIdx.x / 64; item < items;
+         item += step) {
+        const uint32_t v = div_by(item, slices);
+        const int col = (int)((item - v * slices.d) * 64 + threadIdx.x % 64) * 4;
+        if (col >= C) continue;
+        const Run run = run_of(starts, v);
+        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+        if (!run.none) {
+            if (run.first == run.last || run.last - run.first >= kLongRun) continue;
+            sum = load4(tail + (size_t)run.first * C, col, C);
+            constexpr int U = 8;
+            for (uint32_t c0 = run.first + 1; c0 <= run.last; c0 += U) {
+                f32x4 p[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    p[u] = c0 + u <= run.last ? load4(head + (size_t)(c0 + u) * C, col, C)
+                                              : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int u = 0; u < U; ++u) sum += p[u];
+            }
+            sum *= scale;
+        }
+        const float v4[4] = {sum[0], sum[1], sum[2], sum[3]};
+        store_floats(dtable + (size_t)v * C, col, C, v4);
+    }
+}
+
+// A run over more than kLongRun chunks holds a multiple of kLongRun after its first chunk: block
+// b looks at chunk b * kLongRun, and the first one of a run sums it, 16 waves taking its chunks in
+// turn.
+constexpr int kLongWaves = 16;
+__global__ __launch_bounds__(64 * kLongWaves) void embed_join_long_kernel(
+    const uint32_t* __restrict__ keys, const float* __restrict__ head,
+    const float* __restrict__ tail, const uint32_t* __restrict__ starts,
+    float* __restrict__ dtable, uint32_t V, int C, float scale) {
+    __shared__ f32x4 part[kLongWaves][64];
+    const uint32_t at = (blockIdx.x + 1) * kLongRun;
+    const uint32_t v = keys[(size_t)at * kChunk];
+    if (v >= V) return;
+    const Run run = run_of(starts, v);
+    if (run.last - run.first < kLongRun || at - run.first > kLongRun || at == run.first) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int col = (int)(blockIdx.y * 64 + lane) * 4;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    if (col < C) {
+        if (wave == 0) sum = load4(tail + (size_t)run.first * C, col, C);
+        constexpr int U = 8;
+        for (uint32_t c0 = run.first + 1 + wave; c0 <= run.last; c0 += U * kLongWaves) {
+            f32x4 p[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const uint32_t c = c0 + u * kLongWaves;
+                p[u] = c <= run.last ? load4(head + (size_t)c * C, col, C)
+                                     : f32x4{0.f, 0.f, 0.f, 0.f};
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) sum += p[u];
+        }
+    }
+    part[wave][lane] = sum;
+    __syncthreads();
+    if (wave == 0 && col < C) {
+        for (int w = 1; w < kLongWaves; ++w) sum += part[w][lane];
+        sum *= scale;
+        const float v4[4] = {sum[0], sum[1], sum[2], sum[3]};
+        store_floats(dtable + (size_t)v * C, col, C, v4);
+    }
+}
+
+__global__ __launch_bounds__(kThreads) void embed_zero_kernel(float* __restrict__ p, size_t n) {
+    for (size_t i = (size_t)blockIdx.x * kThreads + threadIdx.x; i < n;
+         i += (size_t)gridDim.x * kThreads)
+        p[i] = 0.f;
+}
+
+// ---------------------------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------------------------
+// A launch holds fewer than 2^32 threads: kernels whose work can be more loop over it.
+constexpr int64_t kMaxBlocks = 1 << 22;
+size_t pad256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+// What the gradient keeps in its workspace, as offsets in bytes.
+struct BwdPlan {
+    bool ranked;
+    int passes;
+    int64_t tiles, chunks;
+    size_t keys[2], order[2], counts, totals, starts, head, tail, bytes;
+};
+BwdPlan bwd_plan(int64_t M, int64_t V, int64_t C) {
+    BwdPlan p = {};
+    p.ranked = M <= kRankMax;
+    p.passes = 1;
+    while ((V >> (8 * p.passes)) != 0) ++p.passes;  // keys are 0 .. V
+    p.tiles = up(M, kTile);
+    p.chunks = up(M, kChunk);
+    size_t at = 0;
+    const auto take = [&](size_t n) {
+        const size_t here = at;
+        at += pad256(n);
+        return here;
+    };
+    const int copies = p.ranked || p.passes == 1 ? 1 : 2;
+    for (int i = 0; i < copies; ++i) {
+        p.keys[i] = take((size_t)M * 4);
+        p.order[i] = take((size_t)M * 4);
+    }
+    if (!p.ranked) {
+        p.counts = take((size_t)p.tiles * kDigits * 4);
+        p.totals = take(kDigits * 4);
+    }
+    p.starts = take((size_t)(V + 1) * 4);
+    p.head = take((size_t)p.chunks * C * 4);
+    p.tail = take((size_t)p.chunks * C * 4);
+    p.bytes = at;
+    return p;
+}
+
+clk_status validate(const char* who, clk_dtype dtype, clk_dtype ids_dtype, int64_t M, int64_t V,
+                    int64_t C) {
+    if (dtype != CLK_F16 && dtype != CLK_BF16 && dtype != CLK_F32)
+        return fail(CLK_INVALID_ARGUMENT, "%s: dtype %s not supported (f16, bf16, f32)", who,
+                    dtype_name(dtype));
+    if (ids_dtype != CLK_S32 && ids_dtype != CLK_S64)
+        return fail(CLK_INVALID_ARGUMENT, "%s: ids of type %s not supported (s32, s64)", who,
+                    dtype_name(ids_dtype));
+    if (M < 0 || V < 0 || C <= 0)
+        return fail(CLK_INVALID_ARGUMENT, "%s: ids [M], table [V,C] with C > 0 expected", who);
+    // These keep token, row and chunk numbers in 31 bits and a launch's threads in 32.
+    if (M > (1 << 30) || V > (1 << 30) - 1 || C > (1 << 20) || M * C > ((int64_t)1 << 38) ||
+        V * C > ((int64_t)1 << 37))
+        return fail(CLK_INVALID_ARGUMENT, "%s: M=%lld, [V,C] = [%lld,%lld] too large", who,
+                    (long long)M, (long long)V, (long long)C);
+    return CLK_OK;
+}
+
+template <typename TR, typename ID>
+void launch_fwd(hipStream_t st, const void* table, const void* ids, void* out, int64_t M,
+                int64_t V, int64_t C, float scale) {
+    using E = typename TR::elem;
+    constexpr int N = Vec<TR>::N;
+    const bool whole = C % N == 0;
+    const int64_t nvec = up(C, N);
+    // About four vectors a thread.
+    const int rows = (int)std::max<int64_t>(1, 4 * kThreads / nvec);
+    const int grid = (int)std::min<int64_t>(up(M, rows), kMaxBlocks);
+    KernelTimer timer("embedding", st);
+    const auto kernel = whole ? embed_kernel<TR, ID, true> : embed_kernel<TR, ID, false>;
+    kernel<<<grid, kThreads, 0, st>>>(static_cast<const E*>(table), static_cast<const ID*>(ids),
+                                      static_cast<E*>(out), M, V, (int)C, rows,
+                                      fast_div((uint32_t)nvec), scale);
+}
+
+template <typename ID>
+void sort_tokens(hipStream_t st, const ID* ids, char* ws, const BwdPlan& p, int64_t M, int64_t V,
+                 uint32_t** keys, uint32_t** order) {
+    const auto at = [&](size_t off) { return reinterpret_cast<uint32_t*>(ws + off); };
+    if (p.ranked) {
+        *keys = at(p.keys[0]);
+        *order = at(p.order[0]);
+        KernelTimer timer("embedding_bwd_rank", st);
+        embed_rank_kernel<ID><<<(int)up(M, kRankTokens), kThreads, 0, st>>>(ids, (int)M,
+                                                                            (uint32_t)V, *keys,
+                                                                            *order);
+        return;
+    }
+    for (int pass = 0; pass < p.passes; ++pass) {
+        uint32_t *to_keys = at(p.keys[pass & 1]), *to_order = at(p.order[pass & 1]);
+        const auto run = [&](auto src) {
+            KernelTimer timer("embedding_bwd_sort", st);
+            embed_count_kernel<<<(int)p.tiles, kThreads, 0, st>>>(src, M, 8 * pass, p.tiles,
+                                                                  at(p.counts));
+            embed_scan_kernel<<<kDigits, kThreads, 0, st>>>(at(p.counts), p.tiles, at(p.totals));
+            embed_scatter_kernel<<<(int)p.tiles, kThreads, 0, st>>>(
+                src, M, 8 * pass, p.tiles, at(p.counts), at(p.totals), to_keys, to_order);
+        };
+        if (pass == 0) run(FirstKeys<ID>{ids, (uint32_t)V});
+        else run(NextKeys{*keys, *order});
+        *keys = to_keys;
+        *order = to_order;
+    }
+}
+
+template <typename TR, int LPR>
+void launch_sum(hipStream_t st, const void* dout, const uint32_t* keys, const uint32_t* order,
+                float* dtable, char* ws, const BwdPlan& p, int64_t M, int64_t V, int64_t C,
+                float scale) {
+    using E = typename TR::elem;
+    constexpr int N = Vec<TR>::N;
+    const int64_t slices = up(up(C, N), LPR);
+    const int64_t sum_blocks = up(p.chunks * slices, kThreads / LPR);
+    const int64_t grid = sum_blocks + up(V + 1, kThreads);
+    const auto kernel = C % N == 0 ? embed_sum_kernel<TR, LPR, true>
+                                   : embed_sum_kernel<TR, LPR, false>;
+    KernelTimer timer("embedding_bwd_sum", st);
+    kernel<<<(uint32_t)grid, kThreads, 0, st>>>(
+        static_cast<const E*>(dout), keys, order, dtable, reinterpret_cast<float*>(ws + p.head),
+        reinterpret_cast<float*>(ws + p.tail), reinterpret_cast<uint32_t*>(ws + p.starts),
+        (uint32_t)M, (uint32_t)V, (int)C, (uint32_t)p.chunks, fast_div((uint32_t)slices),
+        (uint32_t)sum_blocks, scale);
+}
+
+template <typename TR, typename ID>
+void launch_bwd(hipStream_t st, const void* dout, const void* ids, float* dtable, char* ws,
+                int64_t M, int64_t V, int64_t C, float scale) {
+    constexpr int N = Vec<TR>::N;
+    const BwdPlan p = bwd_plan(M, V, C);
+    uint32_t *keys = nullptr, *order = nullptr;
+    sort_tokens<ID>(st, static_cast<const ID*>(ids), ws, p, M, V, &keys, &order);
+    // Lanes a row: as many as it has vectors, up to the 16 that read 256 bytes of it.
+    const int64_t nvec = up(C, N);
+    const auto sum = nvec > 8   ? launch_sum<TR, 16>
+                     : nvec > 4 ? launch_sum<TR, 8>
+                     : nvec > 2 ? launch_sum<TR, 4>
+                                : launch_sum<TR, 2>;
+    sum(st, dout, keys, order, dtable, ws, p, M, V, C, scale);
+    const float* head = reinterpret_cast<const float*>(ws + p.head);
+    const float* tail = reinterpret_cast<const float*>(ws + p.tail);
+    const uint32_t* starts = reinterpret_cast<const uint32_t*>(ws + p.starts);
+    const int64_t slices = up(C, 256);
+    {
+        KernelTimer timer("embedding_bwd_join", st);
+        const int64_t grid = std::min<int64_t>(up(V * slices, kThreads / 64), kMaxBlocks);
+        embed_join_kernel<<<(uint32_t)grid, kThreads, 0, st>>>(
+            head, tail, starts, dtable, (uint32_t)V, (int)C, fast_div((uint32_t)slices), scale);
+    }
+    const int64_t marks = (p.chunks - 1) / kLongRun;  // multiples of kLongRun past chunk 0
+    if (marks > 0) {
+        KernelTimer timer("embedding_bwd_join_long", st);
+        embed_join_long_kernel<<<dim3((uint32_t)marks, (uint32_t)slices), 64 * kLongWaves, 0,
+                                 st>>>(keys, head, tail, starts, dtable, (uint32_t)V, (int)C,
+                                       scale);
+    }
+}
+
+// fn<TR, ID> for the two types of a call.
+#define CLK_EMBED_TYPES(dtype, ids_dtype, fn, ...)                          \
+    do {                                                                    \
+        const bool wide = (ids_dtype) == CLK_S64;                           \
+        if ((dtype) == CLK_BF16)                                            \
+            wide ? fn<BF16, int64_t>(__VA_ARGS__) : fn<BF16, int32_t>(__VA_ARGS__); \
+        else if ((dtype) == CLK_F16)                                        \
+            wide ? fn<F16, int64_t>(__VA_ARGS__) : fn<F16, int32_t>(__VA_ARGS__);   \
+        else                                                                \
+            wide ? fn<F32, int64_t>(__VA_ARGS__) : fn<F32, int32_t>(__VA_ARGS__);   \
+    } while (0)
+
+}  // namespace
+}  // namespace clk
+
+using namespace clk;
+
+extern "C" clk_status clk_embedding_fwd(hipStream_t stream, clk_dtype dtype, const void* table,
+                                        clk_dtype ids_dtype, const void* ids, void* out,
+                                        int64_t M, int64_t V, int64_t C, float scale) {
+    const char* who = "embedding";
+    const clk_status s = validate(who, dtype, ids_dtype, M, V, C);
+    if (s != CLK_OK) return s;
+    if (M == 0) return ok();
+    if ((V > 0 && !table) || !ids || !out)
+        return fail(CLK_INVALID_ARGUMENT, "%s: null pointer", who);
+    if (!aligned16(table) || !aligned16(out))
+        return fail(CLK_INVALID_ARGUMENT, "%s: table and out must be 16-byte aligned", who);
+    CLK_EMBED_TYPES(dtype, ids_dtype, launch_fwd, stream, table, ids, out, M, V, C, scale);
+    return check_launch(who);
+}
+
+extern "C" size_t clk_embedding_bwd_workspace_size(int64_t M, int64_t V, int64_t C) {
+    if (M <= 0 || V <= 0 || C <= 0 || validate("embedding_bwd", CLK_F32, CLK_S32, M, V, C) != CLK_OK)
+        return 0;
+    return bwd_plan(M, V, C).bytes;
+}
+
+extern "C" clk_status clk_embedding_bwd(hipStream_t stream, clk_dtype dtype, const void* dout,
+                                        clk_dtype ids_dtype, const void* ids, float* dtable,
+                                        void* workspace, size_t workspace_bytes, int64_t M,
+                                        int64_t V, int64_t C, float scale) {
+    const char* who = "embedding_bwd";
+    const clk_status s = validate(who, dtype, ids_dtype, M, V, C);
+    if (s != CLK_OK) return s;
+    if (V == 0) return ok();
+    if (!dtable || (M > 0 && (!dout || !ids || !workspace)))
+        return fail(CLK_INVALID_ARGUMENT, "%s: null pointer", who);
+    if (M == 0) {  // no tokens: the gradient is zero
+        const size_t n = (size_t)V * C;
+        embed_zero_kernel<<<(int)std::min<size_t>((n + kThreads - 1) / kThreads, 4096), kThreads,
+                            0, stream>>>(dtable, n);
+        return check_launch(who);
+    }
+    if (!aligned16(dout) || !aligned16(dtable) || !aligned16(workspace))
+        return fail(CLK_INVALID_ARGUMENT,
+                    "%s: dout, dtable and workspace must be 16-byte aligned", who);
+    const size_t need = clk_embedding_bwd_workspace_size(M, V, C);
+    if (workspace_bytes < need)
+        return fail(CLK_INVALID_ARGUMENT, "%s: workspace %zu bytes, needs %zu", who,
+                    workspace_bytes, need);
+    CLK_EMBED_TYPES(dtype, ids_dtype, launch_bwd, stream, dout, ids, dtable,
+                    static_cast<char*>(workspace), M, V, C, scale);
+    return check_launch(who);
+}

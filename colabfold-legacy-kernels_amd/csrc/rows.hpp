@@ -1,0 +1,99 @@
+// Rows of C elements as 16-byte vectors, for the kernels that take any C: WHOLE rows hold whole
+// vectors (C a multiple of Vec::N, so that every vector of a 16-byte aligned array is aligned);
+// otherwise the last vector of a row is partial and rows begin at any element.
+#pragma once
+
+#include <algorithm>
+
+#include "common.hpp"
+
+namespace clk {
+
+template <typename TR>
+struct Vec {
+    static constexpr int N = 16 / sizeof(typename TR::elem);
+};
+
+// The N elements from `col` on, zero past the row's end.
+template <typename TR, bool WHOLE>
+__device__ __forceinline__ u32x4 load_vec(const typename TR::elem* row, int col, int C) {
+    constexpr int N = Vec<TR>::N;
+    if (WHOLE) return ld16(row + col);
+    if (col + N <= C) return ld16_a2(row + col);
+    typename TR::elem e[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) e[i] = col + i < C ? row[col + i] : TR::from_f(0.f);
+    u32x4 raw;
+    __builtin_memcpy(&raw, e, 16);
+    return raw;
+}
+
+template <typename TR>
+__device__ __forceinline__ void unpack_vec(u32x4 raw, float (&out)[Vec<TR>::N]) {
+    typename TR::elem e[Vec<TR>::N];
+    __builtin_memcpy(e, &raw, 16);
+#pragma unroll
+    for (int i = 0; i < Vec<TR>::N; ++i) out[i] = TR::to_f(e[i]);
+}
+
+template <typename TR>
+__device__ __forceinline__ u32x4 pack_vec(const float (&v)[Vec<TR>::N]) {
+    typename TR::elem e[Vec<TR>::N];
+#pragma unroll
+    for (int i = 0; i < Vec<TR>::N; ++i) e[i] = TR::from_f(v[i]);
+    u32x4 raw;
+    __builtin_memcpy(&raw, e, 16);
+    return raw;
+}
+
+// Stores of results that the kernel does not read again (non-temporal where a vector is aligned).
+template <typename TR, bool WHOLE>
+__device__ __forceinline__ void store_vec(typename TR::elem* row, int col, int C, u32x4 raw) {
+    constexpr int N = Vec<TR>::N;
+    if (WHOLE) {
+        __builtin_nontemporal_store(raw, reinterpret_cast<u32x4*>(row + col));
+    } else if (col + N <= C) {
+        *reinterpret_cast<u32x4_a2*>(row + col) = raw;
+    } else {
+        typename TR::elem e[N];
+        __builtin_memcpy(e, &raw, 16);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (col + i < C) row[col + i] = e[i];
+    }
+}
+
+// N floats of a [C] vector from `col` on, at float alignment; `fill` past its end.
+template <int N, bool WHOLE>
+__device__ __forceinline__ void load_floats(const float* p, int col, int C, float fill,
+                                            float (&out)[N]) {
+#pragma unroll
+    for (int q = 0; q < N; q += 4) {
+        if (WHOLE || col + q + 4 <= C) {
+            const f32x4 v = ld4f(p + col + q);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) out[q + i] = v[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) out[q + i] = col + q + i < C ? p[col + q + i] : fill;
+        }
+    }
+}
+
+template <int N>
+__device__ __forceinline__ void store_floats(float* p, int col, int C, const float (&v)[N]) {
+#pragma unroll
+    for (int q = 0; q < N; q += 4) {
+        if (col + q + 4 <= C) {
+            *reinterpret_cast<f32x4_a4*>(p + col + q) = f32x4{v[q], v[q + 1], v[q + 2], v[q + 3]};
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (col + q + i < C) p[col + q + i] = v[q + i];
+        }
+    }
+}
+
+inline int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+}  // namespace clk

@@ -73,6 +73,8 @@ KernelTimer::~KernelTimer() {
 
 const char* dtype_name(clk_dtype t) {
     switch (t) {
+        case CLK_S32: return "s32";
+        case CLK_S64: return "s64";
         case CLK_U8: return "u8";
         case CLK_F16: return "f16";
         case CLK_F32: return "f32";

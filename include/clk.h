@@ -17,6 +17,8 @@
  *              (0 = key absent); lse [N,H,Sq] float32 (natural log)
  *   layer norm x, y [M,C]; scale, offset [C] float32
  *   gdp        x [M,K]; wp, wg [K,N]; bp, bg [N]; mask [M]; out [M,N]
+ *   embedding  table [V,C]; ids [M] int32 or int64; out, dout [M,C]; dtable [V,C] float32
+ *   residual   x, o, gate, r, h [M,C]; the norms' scales and offsets, res_scale [C] float32
  */
 #ifndef CLK_H_
 #define CLK_H_
@@ -38,11 +40,18 @@ typedef enum clk_status {
 } clk_status;
 
 typedef enum clk_dtype {
+    CLK_S32 = 4,
+    CLK_S64 = 5,
     CLK_U8 = 6,
     CLK_F16 = 10,
     CLK_F32 = 11,
     CLK_BF16 = 16,
 } clk_dtype;
+
+typedef enum clk_norm {
+    CLK_NORM_LAYER = 0,
+    CLK_NORM_RMS = 1,
+} clk_norm;
 
 /* Message of the last non-OK status returned on this thread ("" if none). */
 const char* clk_last_error(void);
@@ -321,6 +330,115 @@ clk_status clk_triangle_multiply(hipStream_t stream, clk_dtype dtype, const void
                                  const void* const* b, void* out, void* workspace,
                                  size_t workspace_bytes, int64_t N, int64_t C, int outgoing,
                                  float eps);
+
+/*
+ * Token embedding (new; the residue types, MSA tokens and relative positions that the blocks'
+ * representations begin from): out[i] = scale * table[ids[i]]. An id outside [0, V) is an absent
+ * token: its row of out is zero. table and out of dtype CLK_F16, CLK_BF16 or CLK_F32, 16-byte
+ * aligned; ids of ids_dtype CLK_S32 or CLK_S64. Any C up to 2^20; M and V below 2^30, M*C up to
+ * 2^38, V*C up to 2^37.
+ */
+clk_status clk_embedding_fwd(hipStream_t stream, clk_dtype dtype, const void* table,
+                             clk_dtype ids_dtype, const void* ids, void* out, int64_t M,
+                             int64_t V, int64_t C, float scale);
+
+/*
+ * Its backward: dtable[v] = scale * sum of dout[i] over the tokens with ids[i] = v, float32 [V,C];
+ * rows that no token names are zero, absent tokens add nothing. Deterministic: the tokens are
+ * sorted by row (stably) and summed in a fixed order, no floating-point atomics. dout, dtable and
+ * workspace 16-byte aligned; workspace: clk_embedding_bwd_workspace_size bytes.
+ */
+size_t clk_embedding_bwd_workspace_size(int64_t M, int64_t V, int64_t C);
+clk_status clk_embedding_bwd(hipStream_t stream, clk_dtype dtype, const void* dout,
+                             clk_dtype ids_dtype, const void* ids, float* dtable, void* workspace,
+                             size_t workspace_bytes, int64_t M, int64_t V, int64_t C,
+                             float scale);
+
+/*
+ * Residual join with the norms around it (new): for the residual stream x [M,C] and a block's
+ * output o [M,C],
+ *   u = N_post(o);  t = sigmoid(gate) * u;  r = x + res_scale * t;  h = N_pre(r)
+ * r is the new stream (rounded to the dtype), h the next block's input, normed from the rounded r.
+ * N is a LayerNorm (CLK_NORM_LAYER) or an RMS norm (CLK_NORM_RMS, no mean) over the last axis with
+ * float32 scale [C] and, where given, offset [C]. post_scale NULL: no norm after the block (u = o);
+ * gate NULL: t = u; res_scale NULL: 1; pre_scale NULL: no norm before the next block, and h must be
+ * NULL. x, o, gate, r, h of dtype CLK_F16, CLK_BF16 or CLK_F32, 16-byte aligned.
+ */
+clk_status clk_residual_norm_fwd(hipStream_t stream, clk_dtype dtype, clk_norm norm,
+                                 const void* x, const void* o, const void* gate,
+                                 const float* post_scale, const float* post_offset,
+                                 const float* res_scale, const float* pre_scale,
+                                 const float* pre_offset, void* r, void* h, int64_t M, int64_t C,
+                                 float eps);
+
+/*
+ * Its backward, from r (the forward's result), o and gate: dr is the gradient of r from the
+ * stream's other readers (NULL: zero), dh the gradient of h (with pre_scale, and only with it).
+ * Writes dx, d_o and, with gate, dgate [M,C] in the dtype and the column sums dpost_scale,
+ * dpost_offset, dres_scale, dpre_scale, dpre_offset [C] float32 (each may be NULL; none for a
+ * parameter that is not there). Deterministic. Workspace: clk_residual_norm_bwd_workspace_size
+ * bytes, 16-byte aligned. M = 0 writes zero column sums.
+ */
+size_t clk_residual_norm_bwd_workspace_size(int64_t M, int64_t C);
+clk_status clk_residual_norm_bwd(hipStream_t stream, clk_dtype dtype, clk_norm norm,
+                                 const void* r, const void* o, const void* gate,
+                                 const float* post_scale, const float* post_offset,
+                                 const float* res_scale, const float* pre_scale, const void* dr,
+                                 const void* dh, void* dx, void* d_o, void* dgate,
+                                 float* dpost_scale, float* dpost_offset, float* dres_scale,
+                                 float* dpre_scale, float* dpre_offset, void* workspace,
+                                 size_t workspace_bytes, int64_t M, int64_t C, float eps);
+
+/*
+ * AdamW over many tensors at once (new; it takes the float32 weight gradients of the backward
+ * entries). A tensor: param float32 (the master weights), grad of grad_dtype, the states exp_avg
+ * and exp_avg_sq, and copy, the working copy of the weights in copy_dtype CLK_BF16 or CLK_F16 that
+ * the step writes as well (NULL: none). With 32-bit states both are float32 [numel] and scales is
+ * NULL; with 8-bit ones exp_avg is int8 and exp_avg_sq uint8 [numel], 4-byte aligned, and scales
+ * float32 [ceil(numel / 256)][2] holds each block's largest |exp_avg| and exp_avg_sq, with
+ *   exp_avg = sign(c) * (c / 127)^2 * scales[.][0],  exp_avg_sq = (c / 255)^4 * scales[.][1].
+ * All zero bytes are zero states. Arrays other than the codes need their elements' alignment only.
+ */
+typedef struct clk_adamw_tensor {
+    float* param;
+    const void* grad;
+    void* exp_avg;
+    void* exp_avg_sq;
+    float* scales;
+    void* copy;
+    int64_t numel;
+    clk_dtype grad_dtype;
+    clk_dtype copy_dtype;
+} clk_adamw_tensor;
+
+/*
+ * Host only: checks the tensors, writes the number of table entries (64 bytes each) to *chunks and,
+ * unless table is NULL, the table to host memory; the caller copies it to the device and keeps it
+ * as long as the tensors stay where they are. Buffers that a step writes may not overlap others
+ * (gradients may be shared).
+ */
+clk_status clk_adamw_table(const clk_adamw_tensor* tensors, int64_t n, int state_bits,
+                           void* table, size_t table_bytes, int64_t* chunks);
+
+/*
+ * One step (the step-th, from 1) over the tensors of a table in device memory:
+ *   g = grad * grad_scale;  m = beta1*m + (1 - beta1)*g;  v = beta2*v + (1 - beta2)*g*g
+ *   p = p*(1 - lr*weight_decay) - lr/(1 - beta1^step) * m / (sqrt(v)/sqrt(1 - beta2^step) + eps)
+ * hyper (NULL: none) is a float32 [4] in device memory, {lr, 1 - beta1^step, 1 - beta2^step,
+ * grad_scale}, read when the kernel runs in place of step, lr and grad_scale: a captured graph can
+ * then be replayed with other values. With 8-bit states a block of 256 elements that holds an
+ * infinite or NaN state becomes NaN as a whole.
+ */
+clk_status clk_adamw_step(hipStream_t stream, const void* table, int64_t chunks, int state_bits,
+                          int64_t step, double lr, double beta1, double beta2, double eps,
+                          double weight_decay, double grad_scale, const float* hyper);
+
+/*
+ * The states of a table's tensors as float32, in flat buffers in which tensor i begins at the sum
+ * of the earlier tensors' sizes, each rounded up to 256 elements; zeros in between.
+ */
+clk_status clk_adamw_states(hipStream_t stream, const void* table, int64_t chunks, int state_bits,
+                            float* exp_avg, float* exp_avg_sq);
 
 #ifdef __cplusplus
 } /* extern "C" */

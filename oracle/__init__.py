@@ -17,6 +17,10 @@ gate          the attention output gate O * sigmoid(x.Wg + bg) (no reference cod
               jnp step after the attention targets)
 triangle      the triangle-multiplication contraction, outgoing and incoming (no reference code:
               the step after the gated dual projection)
+embedding     rows of a token table and the table's gradient
+residual_norm a block's output normed, gated, scaled and joined with the residual stream, and the
+              norm before the next block, forward and backward
+adamw         one AdamW step, and the codes of 8-bit states
 evoformer     the pair micro-block composed from the three (LN -> GDP, LN -> bias -> attention)
 
 How each function is pinned (tests/test_oracle.py): against independent textbook routines
@@ -28,6 +32,8 @@ golden vectors or tests for this path, and its CUDA/CUTLASS/XLA build cannot run
 reference binary is used.
 """
 
-from . import attention, layer_norm, gdp, gate, triangle, evoformer  # noqa: F401
+from . import (adamw, attention, embedding, evoformer, gate, gdp, layer_norm,  # noqa: F401
+               residual_norm, triangle)
 
-__all__ = ["attention", "layer_norm", "gdp", "gate", "triangle", "evoformer"]
+__all__ = ["attention", "layer_norm", "gdp", "gate", "triangle", "embedding", "residual_norm",
+           "adamw", "evoformer"]
