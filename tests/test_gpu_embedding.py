@@ -1,0 +1,196 @@
+"""Token embedding and its gradient against the float64 oracle.
+
+Tolerances. Forward: a float32 product and one rounding to the type t, so at most half a step of
+each, relative to the value: eps(t)/2 + 2^-24, and half a smallest subnormal below the normal range.
+Gradient: a float32 sum of n terms in any order is off by at most (n - 1) 2^-24 times the sum of
+their magnitudes; the scale's rounding and its product add two more."""
+import numpy as np
+import pytest
+import torch
+
+from _util import np64
+from colabfold_legacy_kernels import _native, ops
+from oracle import embedding as ref
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+U32 = 2.0 ** -24
+
+
+def make_ids(m, v, law, g, dtype, absent=0.0):
+    if law == "uniform":
+        ids = (torch.rand(m, generator=g) * v).long().clamp(max=v - 1)
+    elif law == "long_tail":
+        ids = torch.exp(torch.rand(m, generator=g) * np.log(v)).long().sub(1).clamp(0, v - 1)
+    elif law == "one":
+        ids = torch.full((m,), v // 2)
+    else:  # sorted runs
+        ids = torch.arange(m) * v // max(m, 1)
+    if absent:
+        bad = torch.tensor([-1, v, -2 ** 31, 2 ** 31 - 1])[torch.randint(0, 4, (m,), generator=g)]
+        ids = torch.where(torch.rand(m, generator=g) < absent, bad, ids)
+    return ids.to(dtype)
+
+
+def check_forward(out, table, ids, scale):
+    want = ref.embedding(np64(table), ids.cpu().numpy(), scale)
+    half = torch.finfo(table.dtype).eps / 2 + U32 + 2.0 ** -23 * (scale != 1.0)
+    tiny = torch.finfo(table.dtype).smallest_normal * torch.finfo(table.dtype).eps / 2
+    err = np.abs(np64(out) - want)
+    assert (err <= half * np.abs(want) + tiny).all(), float((err - half * np.abs(want)).max())
+
+
+def check_gradient(got, dout, ids, rows, scale):
+    d, i = np64(dout), ids.cpu().numpy()
+    want = ref.embedding_bwd(d, i, rows, scale)
+    size = ref.embedding_bwd(np.abs(d), i, rows, abs(scale))
+    count = np.bincount(i[(i >= 0) & (i < rows)].reshape(-1), minlength=rows)[:, None]
+    err = np.abs(np64(got) - want)
+    assert (err <= (count + 3) * U32 * size + 1e-37).all(), float((err / (size + 1e-30)).max())
+    assert not np64(got)[count[:, 0] == 0].any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,v,c", [(1, 1, 1), (3, 2, 7), (64, 22, 256), (129, 65, 128), (7, 5, 8),
+                                   (1000, 300, 449), (33, 9, 24), (5, 4, 20000), (300, 11, 3)])
+def test_forward(cuda, dtype, m, v, c):
+    g = torch.Generator().manual_seed(m + c)
+    table = torch.randn(v, c, generator=g).to(dtype).to(cuda)
+    for idt in (torch.int32, torch.int64):
+        ids = make_ids(m, v, "uniform", g, idt, 0.2).to(cuda)
+        for scale in (1.0, 11.25, 0.3):
+            check_forward(ops.embedding(table, ids, scale), table, ids, scale)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("law", ["uniform", "long_tail", "one", "runs"])
+@pytest.mark.parametrize("m,v,c", [
+    (1, 1, 1), (1, 9, 16), (31, 3, 8), (32, 3, 8), (33, 3, 8), (64, 22, 256), (257, 300, 129),
+    (1500, 65, 128), (8192, 40, 24), (8193, 65, 64), (9000, 255, 40), (9000, 256, 40),
+    (20000, 70000, 12), (70000, 23, 36), (5000, 2, 1100)])
+def test_gradient(cuda, dtype, law, m, v, c):
+    g = torch.Generator().manual_seed(m + v + c)
+    dout = torch.randn(m, c, generator=g).to(dtype).to(cuda)
+    ids = make_ids(m, v, law, g, torch.int64 if m % 2 else torch.int32, 0.1).to(cuda)
+    got = ops.embedding_bwd(dout, ids, v, 1.5)
+    check_gradient(got, dout, ids, v, 1.5)
+    assert torch.equal(got, ops.embedding_bwd(dout, ids, v, 1.5))  # the same bits again
+
+
+@pytest.mark.parametrize("m", [40, 30000])
+def test_gradient_of_absent_tokens_only(cuda, m):
+    dout = torch.full((m, 16), float("nan"), device=cuda, dtype=torch.bfloat16)
+    ids = torch.full((m,), -1, device=cuda)
+    assert torch.equal(ops.embedding_bwd(dout, ids, 7), torch.zeros(7, 16, device=cuda))
+    # Absent among others: what their rows of dout hold reaches nothing.
+    dout[::2] = 1
+    ids[::2] = 3
+    got = ops.embedding_bwd(dout, ids, 7)
+    assert (got[3] == (m + 1) // 2).all() and got.sum() == 16 * ((m + 1) // 2)
+
+
+def test_special_values(cuda):
+    table = torch.tensor([[float("inf"), -0.0, float("nan"), 65504.0]], device=cuda).half()
+    ids = torch.tensor([0, 5, -1], device=cuda)
+    out = ops.embedding(table, ids, 2.0)
+    assert out[0, 0] == float("inf") and out[0, 2].isnan() and out[0, 3] == float("inf")
+    assert not out[1:].any()
+    assert not ops.embedding(table, ids, float("inf"))[1:].any()
+    # A NaN gradient stays in its row.
+    dout = torch.ones(4, 8, device=cuda)
+    dout[1] = float("nan")
+    got = ops.embedding_bwd(dout, torch.tensor([0, 1, 2, 2], device=cuda), 4, 3.0)
+    assert got[1].isnan().all()
+    assert torch.equal(got[[0, 2, 3]], torch.tensor([3.0, 6.0, 0.0], device=cuda)[:, None].expand(3, 8))
+
+
+def test_shapes_and_empty(cuda):
+    table = torch.randn(6, 16, device=cuda)
+    ids = torch.randint(0, 6, (2, 3, 5), device=cuda)
+    out = ops.embedding(table, ids)
+    assert out.shape == (2, 3, 5, 16) and torch.equal(out, table[ids])
+    none = torch.empty(0, dtype=torch.int64, device=cuda)
+    assert ops.embedding(table, none).shape == (0, 16)
+    got = ops.embedding_bwd(torch.empty(0, 16, device=cuda), none, 6)
+    assert torch.equal(got, torch.zeros(6, 16, device=cuda))
+    assert ops.embedding_bwd(out, ids, 0).shape == (0, 16)
+    assert not ops.embedding(table[:0], ids).any()
+    one = torch.tensor(4, device=cuda)
+    assert torch.equal(ops.embedding(table, one), table[4])
+
+
+def test_refusals(cuda):
+    table, ids = torch.randn(6, 16, device=cuda), torch.zeros(4, dtype=torch.int64, device=cuda)
+    dout = torch.randn(4, 16, device=cuda)
+    bad = [lambda: ops.embedding(table.double(), ids), lambda: ops.embedding(table, ids.short()),
+           lambda: ops.embedding(table.t(), ids), lambda: ops.embedding(table[0], ids),
+           lambda: ops.embedding(table.reshape(-1)[4:84].reshape(5, 16)[:, 1:], ids),
+           lambda: ops.embedding(table.reshape(-1)[1:81].reshape(5, 16), ids),  # misaligned
+           lambda: ops.embedding(table, ids.cpu()), lambda: ops.embedding_bwd(dout, ids[:3], 6),
+           lambda: ops.embedding_bwd(dout, ids.float(), 6),
+           lambda: ops.embedding_bwd(dout.double(), ids, 6),
+           lambda: ops.embedding_bwd(dout, ids, -1),
+           lambda: ops.embedding_bwd(dout.t().contiguous().t(), ids, 6)]
+    for call in bad:
+        with pytest.raises(ops.InvalidArgument):
+            call()
+
+
+@pytest.mark.parametrize("m,v,c", [(50, 30, 33), (9001, 300, 64), (70, 3, 128)])
+def test_writes_stay_in_their_buffers(cuda, m, v, c):
+    """Guard bytes behind the table's gradient and the workspace, and around out, stay."""
+    g = torch.Generator().manual_seed(4)
+    lib, st = _native.lib(), torch.cuda.current_stream(cuda).cuda_stream
+    ids = make_ids(m, v, "long_tail", g, torch.int32, 0.1).to(cuda)
+    dout = torch.randn(m, c, generator=g).to(cuda)
+    need = lib.clk_embedding_bwd_workspace_size(m, v, c)
+    ws = torch.full((need + 512,), 0xA5, dtype=torch.uint8, device=cuda)
+    dt = torch.full((v * c + 64,), 7.5, device=cuda)
+    assert lib.clk_embedding_bwd(st, _native.F32, dout.data_ptr(), _native.S32, ids.data_ptr(),
+                                 dt.data_ptr(), ws.data_ptr(), need, m, v, c, 1.0) == _native.OK
+    assert (ws[need:] == 0xA5).all() and (dt[v * c:] == 7.5).all()
+    check_gradient(dt[:v * c].reshape(v, c), dout, ids, v, 1.0)
+    out = torch.full((m * c + 64,), 7.5, device=cuda)
+    table = torch.randn(v, c, generator=g).to(cuda)
+    assert lib.clk_embedding_fwd(st, _native.F32, table.data_ptr(), _native.S32, ids.data_ptr(),
+                                 out.data_ptr(), m, v, c, 1.0) == _native.OK
+    assert (out[m * c:] == 7.5).all()
+
+
+def test_offsets_past_32_bits(cuda):
+    """A table, an output and a gradient of more than 2^31 elements; rows of both ends."""
+    v, c = 2_200_000, 1024
+    table = torch.empty(v, c, dtype=torch.bfloat16, device=cuda)
+    far = torch.tensor([0, 1, v // 2, v - 2, v - 1], device=cuda)
+    rows = torch.randn(5, c, device=cuda).bfloat16()
+    table[far] = rows
+    assert torch.equal(ops.embedding(table, far), rows)
+    ids = torch.zeros(v, dtype=torch.int32, device=cuda)
+    ids[far] = far.int()
+    out = ops.embedding(table, ids)
+    assert torch.equal(out[far], rows) and torch.equal(out[v - 5:v - 2], rows[:1].expand(3, c))
+    del table
+    out.zero_()
+    out[far] = rows
+    got = ops.embedding_bwd(out, ids, v)
+    assert torch.equal(got[far], rows.float()) and not got[2:v // 2].any()
+
+
+def test_autograd_and_streams(cuda):
+    table = torch.randn(40, 64, device=cuda, dtype=torch.bfloat16, requires_grad=True)
+    ids = torch.randint(-1, 40, (50, 3), device=cuda)
+    dout = torch.randn(50, 3, 64, device=cuda).bfloat16()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        y = ops.EmbeddingFunction.apply(table, ids, 8.0)
+        grad, = torch.autograd.grad(y, table, dout)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(y, ops.embedding(table.detach(), ids, 8.0))
+    assert grad.dtype == torch.bfloat16
+    assert torch.equal(grad, ops.embedding_bwd(dout, ids, 40, 8.0).bfloat16())
+    # A gradient that is not contiguous (an expanded one).
+    y = ops.EmbeddingFunction.apply(table, ids, 8.0)
+    grad, = torch.autograd.grad(y.sum(), table)
+    assert torch.equal(grad, ops.embedding_bwd(torch.ones_like(dout), ids, 40, 8.0).bfloat16())
