@@ -432,6 +432,270 @@ __global__ __launch_bounds__(64 * kLongWaves) void embed_join_long_kernel(
     }
 }
 
+// ---------------------------------------------------------------------------------------------
+// Tables of few rows: the gradient is the product onehot(ids)^T . dout on the matrix cores, with
+// float32 sums. No token is sorted and dout is read once, in order. A wave keeps every row of its
+// 64 columns in registers (VT tiles of 16 rows x 4 tiles of 16 columns). A block's 8 waves take WC
+// groups of columns and, 8/WC at a time, steps of 32 tokens; their sums are joined in LDS in the
+// order of the waves and leave as one partial [V, C] a block, which embed_parts_kernel adds up.
+//
+// Neither operand goes through LDS. Lane (r16, g) of an MFMA holds eight tokens (8g + j) of row r16
+// of A and of column r16 of B. As A it compares the ids of its tokens with its row; as B it loads
+// columns 4*r16 .. +3 of each of its tokens, which are the four column tiles' operands once the
+// token pairs are interleaved: tile ct then stands for the columns 4*r16 + ct.
+//
+// 0 * NaN and 0 * infinity would reach other rows: a wave whose sums are not all finite at the end
+// adds its tokens up one by one instead.
+// ---------------------------------------------------------------------------------------------
+constexpr int kStep = 32, kHotWaves = 8, kHotCols = 64;
+constexpr int kHotRows = 144;  // most rows of a table that takes this path
+
+template <typename ID>
+__device__ __forceinline__ int hot_id(ID id) {
+    return id >= 0 && id < (ID)kHotRows ? (int)id : -1;
+}
+
+// Tokens t .. t + 7 of a lane.
+template <typename ID>
+__device__ __forceinline__ void load_ids8(const ID* ids, int64_t t, int64_t end, int (&id)[8]) {
+    typedef ID ID4 __attribute__((ext_vector_type(4), aligned(sizeof(ID))));
+    if (t + 8 <= end) {
+        const ID4 a = *reinterpret_cast<const ID4*>(ids + t);
+        const ID4 b = *reinterpret_cast<const ID4*>(ids + t + 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) id[j] = hot_id(a[j]), id[4 + j] = hot_id(b[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) id[j] = t + j < end ? hot_id(ids[t + j]) : -1;
+    }
+}
+
+// Four columns of a row, zero past its end.
+template <typename TR>
+struct Four {
+    typename TR::elem e[4];
+};
+template <typename TR, bool WHOLE>
+__device__ __forceinline__ Four<TR> load_four(const typename TR::elem* row, int col, int C) {
+    using E = typename TR::elem;
+    typedef unsigned int raw_t
+        __attribute__((ext_vector_type(sizeof(E)), aligned(WHOLE ? 4 * sizeof(E) : sizeof(E))));
+    Four<TR> f;
+    if (WHOLE || col + 4 <= C) {
+        const raw_t raw = *reinterpret_cast<const raw_t*>(row + col);
+        __builtin_memcpy(&f, &raw, sizeof(f));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f.e[i] = col + i < C ? row[col + i] : TR::from_f(0.f);
+    }
+    return f;
+}
+
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+
+// One step of 32 tokens: acc[v][ct] += onehot . columns.
+template <typename TR, int VT>
+__device__ __forceinline__ void hot_step(const int (&id)[8], const Four<TR> (&x)[8], int r16,
+                                         f32x4 (&acc)[VT][4]) {
+    if constexpr (sizeof(typename TR::elem) == 2) {
+        using V8 = typename TR::vec8;
+        V8 b[4];
+#pragma unroll
+        for (int ct = 0; ct < 4; ++ct)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) b[ct][j] = x[j].e[ct];
+        u16x2 ids[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            ids[q] = u16x2{(unsigned short)id[2 * q], (unsigned short)id[2 * q + 1]};
+        const unsigned short one = (unsigned short)kOnePair<TR>;
+#pragma unroll
+        for (int v = 0; v < VT; ++v) {
+            // 1 - |id ^ row|, saturated at 0, is whether they are equal; times the bits of 1.
+            const unsigned short row = (unsigned short)(16 * v + r16);
+            u16x2 a[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                a[q] = __builtin_elementwise_sub_sat(u16x2{1, 1}, ids[q] ^ u16x2{row, row}) *
+                       u16x2{one, one};
+            V8 av;
+            __builtin_memcpy(&av, a, 16);
+#pragma unroll
+            for (int ct = 0; ct < 4; ++ct) acc[v][ct] = TR::mfma(av, b[ct], acc[v][ct]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int v = 0; v < VT; ++v) {
+                const float a = id[j] == 16 * v + r16 ? 1.f : 0.f;
+#pragma unroll
+                for (int ct = 0; ct < 4; ++ct)
+                    acc[v][ct] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, x[j].e[ct], acc[v][ct], 0,
+                                                                      0, 0);
+            }
+    }
+}
+
+template <typename TR, typename ID, int VT, int WC, bool WHOLE>
+__global__ __launch_bounds__(64 * kHotWaves) void embed_hot_kernel(
+    const typename TR::elem* __restrict__ dout, const ID* __restrict__ ids,
+    float* __restrict__ out, size_t part_stride, int64_t M, int V, int C, int64_t tokens,
+    float scale) {
+    constexpr int WT = kHotWaves / WC;
+    constexpr int LD = kHotCols + 4;
+    __shared__ __attribute__((aligned(16))) float red[kHotWaves][16][LD];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r16 = lane & 15, g = lane >> 4;
+    const int cbase = (int)blockIdx.y * kHotCols * WC;
+    const int col = cbase + (wave % WC) * kHotCols + 4 * r16;
+    const int64_t beg = (int64_t)blockIdx.x * tokens;
+    const int64_t end = M - beg < tokens ? M : beg + tokens;
+    const int64_t first = beg + (wave / WC) * kStep;
+
+    f32x4 acc[VT][4];
+#pragma unroll
+    for (int v = 0; v < VT; ++v)
+#pragma unroll
+        for (int ct = 0; ct < 4; ++ct) acc[v][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    // Steps are wave-uniform, so a step's rows are at a scalar base and 32-bit lane offsets. Lanes
+    // past the last column load the first ones; their sums are not stored.
+    const int lcol = col < C ? col : 0;
+    const auto load = [&](int64_t t0, int(&id)[8], Four<TR>(&x)[8]) {
+        load_ids8(ids, t0 + 8 * g, end, id);
+        const typename TR::elem* base = dout + (size_t)t0 * C;
+        const uint32_t off = (uint32_t)(8 * g * C);
+        if (t0 + kStep <= end) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                x[j] = load_four<TR, WHOLE>(base + (off + (uint32_t)(j * C)), lcol, C);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (t0 + 8 * g + j < end) {
+                    x[j] = load_four<TR, WHOLE>(base + (off + (uint32_t)(j * C)), lcol, C);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[j].e[i] = TR::from_f(0.f);
+                }
+            }
+        }
+    };
+    constexpr int64_t kNext = WT * kStep;
+    if constexpr (VT <= 5) {  // two steps in flight
+        int id0[8], id1[8];
+        Four<TR> x0[8], x1[8];
+        if (first < end) load(first, id0, x0);
+        for (int64_t t0 = first; t0 < end; t0 += 2 * kNext) {
+            if (t0 + kNext < end) load(t0 + kNext, id1, x1);
+            hot_step<TR, VT>(id0, x0, r16, acc);
+            if (t0 + kNext < end) {
+                if (t0 + 2 * kNext < end) load(t0 + 2 * kNext, id0, x0);
+                hot_step<TR, VT>(id1, x1, r16, acc);
+            }
+        }
+    } else {  // no registers for a second one
+        for (int64_t t0 = first; t0 < end; t0 += kNext) {
+            int id[8];
+            Four<TR> x[8];
+            load(t0, id, x);
+            hot_step<TR, VT>(id, x, r16, acc);
+        }
+    }
+
+    bool finite = true;
+#pragma unroll
+    for (int v = 0; v < VT; ++v)
+#pragma unroll
+        for (int ct = 0; ct < 4; ++ct)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                finite = finite && __builtin_fabsf(acc[v][ct][i]) < __builtin_inff();
+    if (__any(!finite)) {
+#pragma unroll
+        for (int v = 0; v < VT; ++v)
+#pragma unroll
+            for (int ct = 0; ct < 4; ++ct) acc[v][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int64_t t0 = first; t0 < end; t0 += WT * kStep)
+            for (int64_t t = t0; t < end && t < t0 + kStep; ++t) {
+                const int id = hot_id(ids[t]);
+                if (id < 0 || col >= C || ((id >> 2) & 3) != g) continue;
+                const Four<TR> x = load_four<TR, WHOLE>(dout + (size_t)t * C, col, C);
+#pragma unroll
+                for (int v = 0; v < VT; ++v)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (id >> 4 == v && (id & 3) == i) {
+#pragma unroll
+                            for (int ct = 0; ct < 4; ++ct) acc[v][ct][i] += TR::to_f(x.e[ct]);
+                        }
+            }
+    }
+
+    // Join the waves of each column group, a tile of 16 rows at a time.
+    float* to = out + (size_t)blockIdx.x * part_stride;
+#pragma unroll
+    for (int v = 0; v < VT; ++v) {
+        if (v > 0) lds_barrier();
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<f32x4*>(&red[wave][4 * g + i][4 * r16]) =
+                f32x4{acc[v][0][i], acc[v][1][i], acc[v][2][i], acc[v][3][i]};
+        lds_barrier();
+        constexpr int Q = kHotCols / 4 * WC;  // vectors of four columns in a row of the block
+        for (int e = threadIdx.x; e < 16 * Q; e += 64 * kHotWaves) {
+            const int row = e / Q, q = e % Q;
+            const int wc = q / (kHotCols / 4), c4 = q % (kHotCols / 4) * 4;
+            f32x4 sum = *reinterpret_cast<const f32x4*>(&red[wc][row][c4]);
+#pragma unroll
+            for (int w = 1; w < WT; ++w)
+                sum += *reinterpret_cast<const f32x4*>(&red[w * WC + wc][row][c4]);
+            if (16 * v + row < V) {
+                const float s4[4] = {sum[0] * scale, sum[1] * scale, sum[2] * scale,
+                                     sum[3] * scale};
+                store_floats<4>(to + (size_t)(16 * v + row) * C, cbase + 4 * q, C, s4);
+            }
+        }
+    }
+}
+
+// dtable = scale * the sum of the partials, n floats each, `stride` apart (a multiple of 4): a
+// block takes 32 of them (one 128-byte line of every partial), 32 groups of 8 lanes the partials in
+// turn.
+__global__ __launch_bounds__(kThreads) void embed_parts_kernel(const float* __restrict__ parts,
+                                                               size_t stride, int nparts,
+                                                               float* __restrict__ dtable,
+                                                               size_t n, float scale) {
+    constexpr int U = 8, G = kThreads / 8;
+    __shared__ __attribute__((aligned(16))) float red[G][36];
+    const int q = threadIdx.x & 7, grp = threadIdx.x >> 3;
+    const size_t at = (size_t)blockIdx.x * 32 + 4 * q;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    if (at < stride) {
+        const float* p = parts + at;
+        for (int b0 = grp; b0 < nparts; b0 += U * G) {
+            f32x4 v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                v[u] = b0 + u * G < nparts
+                           ? *reinterpret_cast<const f32x4*>(p + (size_t)(b0 + u * G) * stride)
+                           : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int u = 0; u < U; ++u) sum += v[u];
+        }
+    }
+    *reinterpret_cast<f32x4*>(&red[grp][4 * q]) = sum;
+    __syncthreads();
+    const size_t mine = (size_t)blockIdx.x * 32 + threadIdx.x;
+    if (threadIdx.x < 32 && mine < n) {
+        float s = red[0][threadIdx.x];
+#pragma unroll
+        for (int i = 1; i < G; ++i) s += red[i][threadIdx.x];
+        dtable[mine] = s * scale;
+    }
+}
+
 __global__ __launch_bounds__(kThreads) void embed_zero_kernel(float* __restrict__ p, size_t n) {
     for (size_t i = (size_t)blockIdx.x * kThreads + threadIdx.x; i < n;
          i += (size_t)gridDim.x * kThreads)
@@ -447,6 +711,12 @@ size_t pad256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // What the gradient keeps in its workspace, as offsets in bytes.
 struct BwdPlan {
+    // Tables of few rows: parts of `tokens` tokens, their partial sums `stride` floats apart.
+    bool hot;
+    int parts;
+    int64_t tokens;
+    size_t stride;
+    // The others.
     bool ranked;
     int passes;
     int64_t tiles, chunks;
@@ -454,6 +724,18 @@ struct BwdPlan {
 };
 BwdPlan bwd_plan(int64_t M, int64_t V, int64_t C) {
     BwdPlan p = {};
+    if (V <= kHotRows) {
+        // As many blocks as CUs, with at least four steps of tokens each.
+        p.hot = true;
+        const int64_t cols = up(C, C > kHotCols ? 2 * kHotCols : kHotCols);
+        const int64_t want = std::max<int64_t>(1, 256 / cols);
+        const int64_t least = 4 * kStep * (C > kHotCols ? kHotWaves / 2 : kHotWaves);
+        p.tokens = up(std::max(up(M, want), std::min(M, least)), kStep) * kStep;
+        p.parts = (int)up(M, p.tokens);
+        p.stride = (size_t)up(V * C, 4) * 4;
+        p.bytes = p.parts > 1 ? p.parts * p.stride * sizeof(float) : 16;
+        return p;
+    }
     p.ranked = M <= kRankMax;
     p.passes = 1;
     while ((V >> (8 * p.passes)) != 0) ++p.passes;  // keys are 0 .. V
@@ -565,11 +847,46 @@ void launch_sum(hipStream_t st, const void* dout, const uint32_t* keys, const ui
         (uint32_t)sum_blocks, scale);
 }
 
+template <typename TR, typename ID, int VT, int WC, bool WHOLE>
+void launch_hot(hipStream_t st, const void* dout, const void* ids, float* dtable, char* ws,
+                const BwdPlan& p, int64_t M, int64_t V, int64_t C, float scale) {
+    using E = typename TR::elem;
+    float* parts = reinterpret_cast<float*>(ws);
+    {
+        KernelTimer timer("embedding_bwd_hot", st);
+        embed_hot_kernel<TR, ID, VT, WC, WHOLE>
+            <<<dim3(p.parts, (uint32_t)up(C, kHotCols * WC)), 64 * kHotWaves, 0, st>>>(
+                static_cast<const E*>(dout), static_cast<const ID*>(ids),
+                p.parts > 1 ? parts : dtable, p.stride, M, (int)V, (int)C, p.tokens,
+                p.parts > 1 ? 1.f : scale);
+    }
+    if (p.parts > 1) {
+        KernelTimer timer("embedding_bwd_parts", st);
+        embed_parts_kernel<<<(uint32_t)up(V * C, 32), kThreads, 0, st>>>(
+            parts, p.stride, p.parts, dtable, (size_t)V * C, scale);
+    }
+}
+
 template <typename TR, typename ID>
 void launch_bwd(hipStream_t st, const void* dout, const void* ids, float* dtable, char* ws,
                 int64_t M, int64_t V, int64_t C, float scale) {
     constexpr int N = Vec<TR>::N;
     const BwdPlan p = bwd_plan(M, V, C);
+    if (p.hot) {
+        const auto pick = [&](auto vt, auto wc) {
+            constexpr int VT = decltype(vt)::value, WC = decltype(wc)::value;
+            return C % 4 == 0 ? launch_hot<TR, ID, VT, WC, true> : launch_hot<TR, ID, VT, WC, false>;
+        };
+        const auto rows = [&](auto wc) {
+            return V <= 32   ? pick(std::integral_constant<int, 2>(), wc)
+                   : V <= 80 ? pick(std::integral_constant<int, 5>(), wc)
+                             : pick(std::integral_constant<int, kHotRows / 16>(), wc);
+        };
+        const auto run = C > kHotCols ? rows(std::integral_constant<int, 2>())
+                                      : rows(std::integral_constant<int, 1>());
+        run(st, dout, ids, dtable, ws, p, M, V, C, scale);
+        return;
+    }
     uint32_t *keys = nullptr, *order = nullptr;
     sort_tokens<ID>(st, static_cast<const ID*>(ids), ws, p, M, V, &keys, &order);
     // Lanes a row: as many as it has vectors, up to the 16 that read 256 bytes of it.
