@@ -618,33 +618,44 @@ def embedding_bwd(dout, ids, rows, scale=1.0):
 
 
 _NORMS = {"layer": _native.NORM_LAYER, "rms": _native.NORM_RMS}
+_ROW_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
 
 
-def _norm_pair(pair, c, name, what):
-    """(scale, offset) of a norm: float32 [C] each, the offset or the whole pair may be None."""
-    if pair is None:
-        return None, None
-    scale, offset = pair
-    _shape_check(scale is not None, what, "%s needs a scale" % name)
-    for t in (scale, offset):
-        if t is not None and (t.shape != (c,) or t.dtype != torch.float32):
-            _fail(what, "%s must be float32 [C]" % name)
-    return scale, offset
-
-
-def _residual_args(rows, vectors, kind, what):
-    """(device, dtype code, norm code, M, C) of the [..., C] operands `rows`, all alike."""
-    index = _require(rows + vectors, what)
+def _residual_args(rows, gate, post, res_scale, pre, kind, what):
+    """(device, dtype code, norm code, M, C, post scale, post offset, pre scale, pre offset) of
+    residual_norm's operands; each tensor is looked at once."""
+    first = rows[0][1]
+    if not isinstance(first, torch.Tensor) or not first.is_cuda or not first.dim():
+        _fail(what, "%s must be a [..., C] tensor on a ROCm device" % rows[0][0])
+    shape, dtype, index = first.shape, first.dtype, first.get_device()
+    c = shape[-1]
+    if dtype not in _ROW_DTYPES:
+        _fail(what, "dtype %s not supported" % dtype)
     if kind not in _NORMS:
         _fail(what, "kind must be 'layer' or 'rms', got %r" % (kind,))
-    first = rows[0][1]
-    _shape_check(first.dim() >= 1, what, "%s must have at least one axis" % rows[0][0])
-    for name, t in rows:
-        if t is not None and (t.shape != first.shape or t.dtype != first.dtype):
+    for name, t in rows + (("gate", gate),):
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor) or t.get_device() != index:
+            _fail(what, "%s must be a tensor on the device of %s" % (name, rows[0][0]))
+        if t.shape != shape or t.dtype != dtype:
             _fail(what, "%s must match %s" % (name, rows[0][0]))
-    code = _dtype_code(first, (_native.F16, _native.BF16, _native.F32), what)
-    c = first.shape[-1]
-    return index, code, _NORMS[kind], first.numel() // c if c else 0, c
+        if not t.is_contiguous():
+            _fail(what, "%s must be contiguous" % name)
+    post_scale, post_offset = post if post is not None else (None, None)
+    pre_scale, pre_offset = pre if pre is not None else (None, None)
+    if (post is not None and post_scale is None) or (pre is not None and pre_scale is None):
+        _fail(what, "a norm needs a scale")
+    for name, t in (("post", post_scale), ("post", post_offset), ("res_scale", res_scale),
+                    ("pre", pre_scale), ("pre", pre_offset)):
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor) or t.get_device() != index:
+            _fail(what, "%s must be on the device of %s" % (name, rows[0][0]))
+        if t.dtype != torch.float32 or t.dim() != 1 or t.numel() != c or not t.is_contiguous():
+            _fail(what, "%s must be float32 [C], contiguous" % name)
+    return (index, _DTYPES[dtype], _NORMS[kind], first.numel() // c if c else 0, c, post_scale,
+            post_offset, pre_scale, pre_offset)
 
 
 def residual_norm(x, o, gate=None, post=None, res_scale=None, pre=None, kind="layer", eps=1e-5):
@@ -653,22 +664,13 @@ def residual_norm(x, o, gate=None, post=None, res_scale=None, pre=None, kind="la
     [..., C] of one dtype (f16, bf16, f32); post and pre: (scale, offset) float32 [C] of a LayerNorm
     or, with kind "rms", of an RMS norm, the offset None where there is none; res_scale float32 [C].
     gate, post, res_scale and pre may each be None: no gate, no norm, 1, no norm."""
-    what = "residual_norm"
-    c = x.shape[-1] if isinstance(x, torch.Tensor) and x.dim() else 0
-    post_scale, post_offset = _norm_pair(post, c, "post", what)
-    pre_scale, pre_offset = _norm_pair(pre, c, "pre", what)
-    index, code, norm, m, c = _residual_args(
-        [("x", x), ("o", o), ("gate", gate)],
-        [("post", post_scale), ("post", post_offset), ("res_scale", res_scale),
-         ("pre", pre_scale), ("pre", pre_offset)], kind, what)
-    if res_scale is not None:
-        _shape_check(res_scale.shape == (c,) and res_scale.dtype == torch.float32, what,
-                     "res_scale must be float32 [C]")
+    (index, code, norm, m, c, post_scale, post_offset, pre_scale, pre_offset) = _residual_args(
+        (("x", x), ("o", o)), gate, post, res_scale, pre, kind, "residual_norm")
     r = torch.empty_like(x)
     h = torch.empty_like(x) if pre_scale is not None else None
     _launch(index, _native.lib().clk_residual_norm_fwd, code, norm, x.data_ptr(), o.data_ptr(),
             _ptr(gate), _ptr(post_scale), _ptr(post_offset), _ptr(res_scale), _ptr(pre_scale),
-            _ptr(pre_offset), r.data_ptr(), _ptr(h), m, c, float(eps))
+            _ptr(pre_offset), r.data_ptr(), _ptr(h), m, c, eps)
     return r, h
 
 
@@ -678,35 +680,26 @@ def residual_norm_bwd(r, o, gate, post, res_scale, pre, dr, dh, kind="layer", ep
     dpost_offset, dres_scale, dpre_scale, dpre_offset), the first three in r's dtype, the others
     float32 [C], None for what was not given."""
     what = "residual_norm_bwd"
-    c = r.shape[-1] if isinstance(r, torch.Tensor) and r.dim() else 0
-    post_scale, post_offset = _norm_pair(post, c, "post", what)
-    pre_scale, pre_offset = _norm_pair(pre, c, "pre", what)
-    index, code, norm, m, c = _residual_args(
-        [("r", r), ("o", o), ("gate", gate), ("dr", dr), ("dh", dh)],
-        [("post", post_scale), ("post", post_offset), ("res_scale", res_scale),
-         ("pre", pre_scale), ("pre", pre_offset)], kind, what)
-    if res_scale is not None:
-        _shape_check(res_scale.shape == (c,) and res_scale.dtype == torch.float32, what,
-                     "res_scale must be float32 [C]")
-    _shape_check((dh is not None) == (pre_scale is not None), what,
-                 "dh is given with pre, and only with it")
-    _shape_check(dr is not None or dh is not None, what, "dr or dh must be given")
+    (index, code, norm, m, c, post_scale, post_offset, pre_scale, pre_offset) = _residual_args(
+        (("r", r), ("o", o), ("dr", dr), ("dh", dh)), gate, post, res_scale, pre, kind, what)
+    if (dh is not None) != (pre_scale is not None):
+        _fail(what, "dh is given with pre, and only with it")
+    if dr is None and dh is None:
+        _fail(what, "dr or dh must be given")
     lib = _native.lib()
     wsb = lib.clk_residual_norm_bwd_workspace_size(m, c)
-    ws = _workspace(r, wsb)
+    ws = r.new_empty(max(wsb, 1), dtype=torch.uint8)
     dx, do = torch.empty_like(r), torch.empty_like(r)
     dgate = torch.empty_like(r) if gate is not None else None
-    # The five column sums share one allocation; each begins at a multiple of 16 bytes.
-    c4 = -(-c // 4) * 4
-    sums = r.new_empty((5, c4), dtype=torch.float32)
-    dpost_scale, dpost_offset, dres, dpre_scale, dpre_offset = (
-        sums[i, :c] if t is not None else None
-        for i, t in enumerate((post_scale, post_offset, res_scale, pre_scale, pre_offset)))
+    vectors = (post_scale, post_offset, res_scale, pre_scale, pre_offset)
+    sums = iter(r.new_empty((5, c), dtype=torch.float32).unbind(0))
+    dpost_scale, dpost_offset, dres, dpre_scale, dpre_offset = [
+        None if t is None else next(sums) for t in vectors]
     _launch(index, lib.clk_residual_norm_bwd, code, norm, r.data_ptr(), o.data_ptr(), _ptr(gate),
             _ptr(post_scale), _ptr(post_offset), _ptr(res_scale), _ptr(pre_scale), _ptr(dr),
             _ptr(dh), dx.data_ptr(), do.data_ptr(), _ptr(dgate), _ptr(dpost_scale),
             _ptr(dpost_offset), _ptr(dres), _ptr(dpre_scale), _ptr(dpre_offset), ws.data_ptr(),
-            wsb, m, c, float(eps))
+            wsb, m, c, eps)
     return dx, do, dgate, dpost_scale, dpost_offset, dres, dpre_scale, dpre_offset
 
 

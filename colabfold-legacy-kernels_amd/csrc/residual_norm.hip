@@ -267,6 +267,26 @@ __global__ __launch_bounds__(block_threads<T>()) void join_bwd_kernel(
     const L lane{(int)(threadIdx.x % T), p.C};
     const int slot = threadIdx.x / T;
     const float inv = 1.f / (float)p.C;
+    // The parameters stay in LDS: in registers they would cost a wave a SIMD's worth of them.
+    constexpr int PW = T * NV * N;  // columns that a team holds, at least C
+    __shared__ __attribute__((aligned(16))) float prm[4][PW];
+    for (int c = threadIdx.x; c < PW; c += block_threads<T>()) {
+        prm[0][c] = p.pre_scale && c < p.C ? p.pre_scale[c] : 0.f;
+        prm[1][c] = p.post_scale && c < p.C ? p.post_scale[c] : 0.f;
+        prm[2][c] = p.post_offset && c < p.C ? p.post_offset[c] : 0.f;
+        prm[3][c] = p.res_scale && c < p.C ? p.res_scale[c] : 1.f;
+    }
+    __syncthreads();
+    const auto from_lds = [&](int k, float (&w)[NV][N]) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int q = 0; q < N; q += 4) {
+                const f32x4 x = *reinterpret_cast<const f32x4*>(&prm[k][lane.col(v) + q]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[v][q + i] = x[i];
+            }
+    };
     float acc[kSums][NV][N];
 #pragma unroll
     for (int k = 0; k < kSums; ++k)
@@ -276,17 +296,33 @@ __global__ __launch_bounds__(block_threads<T>()) void join_bwd_kernel(
             for (int i = 0; i < N; ++i) acc[k][v][i] = 0.f;
     const int64_t beg = (int64_t)blockIdx.x * rows_per_block;
     const int64_t end = p.M - beg < rows_per_block ? p.M : beg + rows_per_block;
+    // The next rows' loads are issued before the current rows' arithmetic.
+    u32x4 nr[NV], no[NV], ng[NV], nd[NV], nh[NV];
+    const auto fetch = [&](int64_t row) {
+        const bool there = row < end;
+        if (p.pre_scale) {
+            lane.load(a.r, row, there, nr);
+            lane.load(a.dh, row, there, nh);
+        }
+        lane.load(a.o, row, there, no);
+        if (a.gate) lane.load(a.gate, row, there, ng);
+        if (a.dr) lane.load(a.dr, row, there, nd);
+    };
+    fetch(beg + slot);
     for (int64_t row0 = beg; row0 < end; row0 += ROWS) {
         const int64_t row = row0 + slot;
         const bool there = row < end;
         u32x4 rr[NV], ro[NV], rg[NV], rd[NV], rh[NV];
-        if (p.pre_scale) {
-            lane.load(a.r, row, there, rr);
-            lane.load(a.dh, row, there, rh);
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            rr[v] = nr[v];
+            ro[v] = no[v];
+            rg[v] = ng[v];
+            rd[v] = nd[v];
+            rh[v] = nh[v];
         }
-        lane.load(a.o, row, there, ro);
-        if (a.gate) lane.load(a.gate, row, there, rg);
-        if (a.dr) lane.load(a.dr, row, there, rd);
+        if (row0 + ROWS < end) fetch(row + ROWS);
+        __atomic_signal_fence(__ATOMIC_SEQ_CST);  // keeps the parameters in LDS, not in registers
 
         float d[NV][N], w[NV][N];  // D
 #pragma unroll
@@ -304,7 +340,7 @@ __global__ __launch_bounds__(block_threads<T>()) void join_bwd_kernel(
             for (int v = 0; v < NV; ++v) unpack_vec<TR>(rr[v], y[v]);
             row_stats<T>(lane, y, p, lds, turn, mean, rstd);
             if (!there) rstd = 0.f;  // eps = 0: a row of zeros has none
-            lane.floats(p.pre_scale, 0.f, w);
+            from_lds(0, w);
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
                 float g[N];
@@ -338,8 +374,8 @@ __global__ __launch_bounds__(block_threads<T>()) void join_bwd_kernel(
             float mean, b[NV][N];
             row_stats<T>(lane, u, p, lds, turn, mean, rstd);
             if (!there) rstd = 0.f;
-            lane.floats(p.post_scale, 0.f, w);
-            lane.floats(p.post_offset, 0.f, b);
+            from_lds(1, w);
+            from_lds(2, b);
 #pragma unroll
             for (int v = 0; v < NV; ++v)
 #pragma unroll
@@ -350,7 +386,7 @@ __global__ __launch_bounds__(block_threads<T>()) void join_bwd_kernel(
         }
         {
             float as[NV][N];
-            lane.floats(p.res_scale, 1.f, as);
+            from_lds(3, as);
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
                 float g[N], dg[N];
@@ -403,8 +439,7 @@ __global__ __launch_bounds__(block_threads<T>()) void join_bwd_kernel(
             for (int v = 0; v < NV; ++v)
                 if (lane.col(v) < p.C) store_floats<N>(out + (size_t)k * C4, lane.col(v), C4, acc[k][v]);
     } else {
-        constexpr int W = T * NV * N;  // columns that a team holds, at least C
-        __shared__ __attribute__((aligned(16))) float red[ROWS][W];
+        __shared__ __attribute__((aligned(16))) float red[ROWS][PW];
 #pragma unroll
         for (int k = 0; k < kSums; ++k) {
             if (k > 0) __syncthreads();
@@ -564,8 +599,10 @@ Team team_of(int64_t nvec, int want) {
     return {t, nvec > t ? 2 : 1};
 }
 
-// Blocks of the backward: four a CU; for long rows one, so that the partial sums stay small.
-int64_t bwd_blocks(int64_t C) { return C <= 4096 ? 1024 : 256; }
+// Blocks of the backward: the three a CU that its registers allow, so that all run at once (with
+// 1024 the last quarter ran alone: 81 us against 72 at [384*384, 128] bf16); one for long rows, so
+// that the partial sums stay small.
+int64_t bwd_blocks(int64_t C) { return C <= 4096 ? 768 : 256; }
 int64_t bwd_rows_per_block(int64_t M, int64_t C, int t) {
     const int64_t slots = t > 64 ? 1 : kThreads / t;
     return slots * up(up(M, slots), bwd_blocks(C));
@@ -628,7 +665,7 @@ void launch_bwd(hipStream_t st, const void* r, const void* o, const void* gate, 
     {
         KernelTimer timer("residual_norm_bwd", st);
         const bool done =
-            with_team(team_of(up(p.C, N), 1), p.C % N == 0, [&](auto t, auto nv, auto w) {
+            with_team(team_of(up(p.C, N), 8 / N), p.C % N == 0, [&](auto t, auto nv, auto w) {
                 constexpr int T = decltype(t)::value;
                 const int64_t rows = bwd_rows_per_block(p.M, p.C, T);
                 nblocks = (int)up(p.M, rows);
