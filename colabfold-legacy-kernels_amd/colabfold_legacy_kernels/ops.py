@@ -773,8 +773,11 @@ class AdamWPlan:
             self.starts.append(self.size)
             self.size += -(-size // _STATE_BLOCK) * _STATE_BLOCK
         self._tensors = lists
-        # Autograd's count of in-place changes, for a graph that saved a weight or its copy.
-        self._changed = [t for t in params + copies if t is not None and not t.is_inference()]
+        # Autograd's count of in-place changes, for a graph that saved a weight or its copy; the
+        # views of a tensor share its count.
+        changed = [t if t._base is None else t._base
+                   for t in params + copies if t is not None and not t.is_inference()]
+        self._changed = list({id(t): t for t in changed}.values())
         lib, chunks = _native.lib(), ctypes.c_int64(0)
         _check(lib.clk_adamw_table(table, n, self.state_bits, None, 0, ctypes.byref(chunks)))
         self.chunks = chunks.value

@@ -34,9 +34,8 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kBlock = 256;  // elements that share two scales: one wave, four elements a lane
 
-// A run of at most one chunk of elements of one tensor; 64 bytes, so a block finds all it needs
-// with one scalar load.
-struct Chunk {
+// A run of at most one chunk of elements of one tensor.
+struct alignas(16) Chunk {
     float* p;
     const void* g;
     void *m, *v;
@@ -47,6 +46,14 @@ struct Chunk {
     uint16_t grad_type, copy_type;  // clk_dtype; copy_type 0: none
 };
 static_assert(sizeof(Chunk) == 64);
+
+// The block's chunk, all 64 bytes in one round of scalar loads (field by field the compiler loads
+// each where it is first needed, one wait after the other).
+__device__ __forceinline__ Chunk load_chunk(const Chunk* table) {
+    typedef unsigned int u32x16 __attribute__((ext_vector_type(16), aligned(16)));
+    const u32x16 raw = *reinterpret_cast<const u32x16*>(table + blockIdx.x);
+    return __builtin_bit_cast(Chunk, raw);
+}
 
 struct Step {
     float b1, omb1, b2, omb2, keep, step, inv_bias2, eps, grad_scale;
@@ -62,120 +69,154 @@ __device__ __forceinline__ void read_hyper(Step& s) {
     s.grad_scale = s.hyper[3];
 }
 
-// Four elements at any element alignment; `cnt` of them exist (the others are zero, and not
-// stored).
+// The pointers of a table come out of memory: said to be global, their accesses need no check for
+// LDS (flat accesses also wait for one another).
+template <typename T>
+using Global = __attribute__((address_space(1))) T*;
+template <typename T>
+__device__ __forceinline__ Global<T> global(const void* p) {
+    return (Global<T>)p;
+}
+
+// Four elements from `at` on of a chunk of n, at any element alignment. FULL: all four exist.
+// Otherwise the missing ones are loaded as the chunk's last and become zero, so that no lane
+// branches around a load (each branch would wait for the loads in it), and are not stored.
+__device__ __forceinline__ uint32_t inside(uint32_t at, uint32_t n) { return at < n ? at : n - 1; }
 typedef unsigned int u32x2_a2 __attribute__((ext_vector_type(2), aligned(2)));
-template <typename TR>
-__device__ __forceinline__ void load_half4(const void* p, uint32_t at, int cnt, float (&x)[4]) {
+template <typename TR, bool FULL>
+__device__ __forceinline__ void load_half4(const void* p, uint32_t at, uint32_t n, float (&x)[4]) {
     using E = typename TR::elem;
-    const E* e = static_cast<const E*>(p) + at;
-    if (cnt >= 4) {
-        const u32x2 raw = *reinterpret_cast<const u32x2_a2*>(e);
+    const auto e = global<const E>(p);
+    if (FULL) {
+        const u32x2 raw = *(Global<const u32x2_a2>)(e + at);
         E h[4];
         __builtin_memcpy(h, &raw, 8);
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[i] = TR::to_f(h[i]);
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = i < cnt ? TR::to_f(e[i]) : 0.f;
+        for (int i = 0; i < 4; ++i) x[i] = TR::to_f(e[inside(at + i, n)]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = at + i < n ? x[i] : 0.f;
     }
 }
-__device__ __forceinline__ void load_float4(const float* p, uint32_t at, int cnt, float (&x)[4]) {
-    if (cnt >= 4) {
-        const f32x4 v = ld4f(p + at);
+template <bool FULL>
+__device__ __forceinline__ void load_float4(const void* p, uint32_t at, uint32_t n, float (&x)[4]) {
+    const auto e = global<const float>(p);
+    if (FULL) {
+        const f32x4 v = *(Global<const f32x4_a4>)(e + at);
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[i] = v[i];
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = i < cnt ? p[at + i] : 0.f;
+        for (int i = 0; i < 4; ++i) x[i] = e[inside(at + i, n)];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = at + i < n ? x[i] : 0.f;
     }
 }
-__device__ __forceinline__ void load_grad4(const Chunk& c, uint32_t at, int cnt, float (&x)[4]) {
-    if (c.grad_type == CLK_F32) load_float4(static_cast<const float*>(c.g), at, cnt, x);
-    else if (c.grad_type == CLK_BF16) load_half4<BF16>(c.g, at, cnt, x);
-    else load_half4<F16>(c.g, at, cnt, x);
+template <bool FULL>
+__device__ __forceinline__ void load_grad4(const Chunk& c, uint32_t at, uint32_t n, float (&x)[4]) {
+    if (c.grad_type == CLK_F32) load_float4<FULL>(c.g, at, n, x);
+    else if (c.grad_type == CLK_BF16) load_half4<BF16, FULL>(c.g, at, n, x);
+    else load_half4<F16, FULL>(c.g, at, n, x);
 }
-__device__ __forceinline__ void store_float4(float* p, uint32_t at, int cnt, const float (&x)[4]) {
-    if (cnt >= 4) {
-        *reinterpret_cast<f32x4_a4*>(p + at) = f32x4{x[0], x[1], x[2], x[3]};
+template <bool FULL>
+__device__ __forceinline__ void store_float4(void* p, uint32_t at, uint32_t n, const float (&x)[4]) {
+    const auto e = global<float>(p) + at;
+    if (FULL) {
+        *(Global<f32x4_a4>)e = f32x4{x[0], x[1], x[2], x[3]};
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (i < cnt) p[at + i] = x[i];
+            if (at + i < n) e[i] = x[i];
     }
 }
-template <typename TR>
-__device__ __forceinline__ void store_half4(void* p, uint32_t at, int cnt, const float (&x)[4]) {
+template <typename TR, bool FULL>
+__device__ __forceinline__ void store_half4(void* p, uint32_t at, uint32_t n, const float (&x)[4]) {
     using E = typename TR::elem;
-    E* e = static_cast<E*>(p) + at;
+    const auto e = global<E>(p) + at;
     E h[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) h[i] = TR::from_f(x[i]);
-    if (cnt >= 4) {
+    if (FULL) {
         u32x2 raw;
         __builtin_memcpy(&raw, h, 8);
-        *reinterpret_cast<u32x2_a2*>(e) = raw;
+        *(Global<u32x2_a2>)e = raw;
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (i < cnt) e[i] = h[i];
+            if (at + i < n) e[i] = h[i];
     }
 }
-__device__ __forceinline__ void store_copy4(const Chunk& c, uint32_t at, int cnt,
+template <bool FULL>
+__device__ __forceinline__ void store_copy4(const Chunk& c, uint32_t at, uint32_t n,
                                             const float (&x)[4]) {
-    if (c.copy_type == CLK_BF16) store_half4<BF16>(c.copy, at, cnt, x);
-    else if (c.copy_type == CLK_F16) store_half4<F16>(c.copy, at, cnt, x);
+    if (c.copy_type == CLK_BF16) store_half4<BF16, FULL>(c.copy, at, n, x);
+    else if (c.copy_type == CLK_F16) store_half4<F16, FULL>(c.copy, at, n, x);
 }
-__device__ __forceinline__ uint32_t load_codes4(const void* p, uint32_t at, int cnt) {
-    const uint8_t* e = static_cast<const uint8_t*>(p) + at;
-    if (cnt >= 4) return *reinterpret_cast<const uint32_t*>(e);
+template <bool FULL>
+__device__ __forceinline__ uint32_t load_codes4(const void* p, uint32_t at, uint32_t n) {
+    const auto e = global<const uint8_t>(p);
+    if (FULL) return *(Global<const uint32_t>)(e + at);
     uint32_t q = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        if (i < cnt) q |= (uint32_t)e[i] << (8 * i);
+        q |= (at + i < n ? (uint32_t)e[inside(at + i, n)] : 0u) << (8 * i);
     return q;
 }
-__device__ __forceinline__ void store_codes4(void* p, uint32_t at, int cnt, uint32_t q) {
-    uint8_t* e = static_cast<uint8_t*>(p) + at;
-    if (cnt >= 4) {
-        *reinterpret_cast<uint32_t*>(e) = q;
+template <bool FULL>
+__device__ __forceinline__ void store_codes4(void* p, uint32_t at, uint32_t n, uint32_t q) {
+    const auto e = global<uint8_t>(p) + at;
+    if (FULL) {
+        *(Global<uint32_t>)e = q;
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (i < cnt) e[i] = (uint8_t)(q >> (8 * i));
+            if (at + i < n) e[i] = (uint8_t)(q >> (8 * i));
     }
 }
 
+// sqrt(x) within 2 ulp: the hardware's root, of a scaled argument where that is too small for it.
+__device__ __forceinline__ float near_sqrt(float x) {
+    const bool small = x < 0x1p-96f;
+    return __builtin_amdgcn_sqrtf(x * (small ? 0x1p64f : 1.f)) * (small ? 0x1p-32f : 1.f);
+}
+// The moments are rounded operation by operation; the weight's step takes the hardware's root and
+// reciprocal (1 ulp each, of a step that is itself a small part of the weight).
 __device__ __forceinline__ void update(const Step& s, float grad, float& p, float& m, float& v) {
     const float g = grad * s.grad_scale;
     m = m * s.b1 + g * s.omb1;
     v = v * s.b2 + (g * s.omb2) * g;
-    p = p * s.keep - m / (sqrtf(v) * s.inv_bias2 + s.eps) * s.step;
+    const float denom = near_sqrt(v) * s.inv_bias2 + s.eps;
+    p = p * s.keep - m * fast_rcp(denom) * s.step;
 }
 
-__device__ __forceinline__ int left(uint32_t n, uint32_t at) {
-    return at < n ? (n - at < 4 ? (int)(n - at) : 4) : 0;
+// A block takes a chunk, a thread four elements of it: all of a chunk's loads are in flight at once
+// (chunks of 4096 elements in four rounds took 94 us instead of 84 for eight blocks' parameters).
+constexpr int kChunk = 4 * kThreads;
+
+template <bool FULL>
+__device__ __forceinline__ void step32(const Chunk& c, const Step& s) {
+    const uint32_t at = 4 * threadIdx.x;
+    float ps[4], gs[4], ms[4], vs[4];
+    load_float4<FULL>(c.p, at, c.n, ps);
+    load_float4<FULL>(c.m, at, c.n, ms);
+    load_float4<FULL>(c.v, at, c.n, vs);
+    load_grad4<FULL>(c, at, c.n, gs);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) update(s, gs[i], ps[i], ms[i], vs[i]);
+    store_float4<FULL>(c.p, at, c.n, ps);
+    store_float4<FULL>(c.m, at, c.n, ms);
+    store_float4<FULL>(c.v, at, c.n, vs);
+    if (c.copy_type) store_copy4<FULL>(c, at, c.n, ps);
 }
 
 __global__ __launch_bounds__(kThreads) void adamw32_kernel(const Chunk* __restrict__ table,
                                                            Step s) {
-    const Chunk c = table[blockIdx.x];
+    const Chunk c = load_chunk(table);
     read_hyper(s);
-    float *m = static_cast<float*>(c.m), *v = static_cast<float*>(c.v);
-    for (uint32_t at = 4 * threadIdx.x; at < c.n; at += 4 * kThreads) {
-        const int cnt = left(c.n, at);
-        float ps[4], gs[4], ms[4], vs[4];
-        load_float4(c.p, at, cnt, ps);
-        load_grad4(c, at, cnt, gs);
-        load_float4(m, at, cnt, ms);
-        load_float4(v, at, cnt, vs);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) update(s, gs[i], ps[i], ms[i], vs[i]);
-        store_float4(c.p, at, cnt, ps);
-        store_float4(m, at, cnt, ms);
-        store_float4(v, at, cnt, vs);
-        if (c.copy_type) store_copy4(c, at, cnt, ps);
-    }
+    if (c.n == kChunk) step32<true>(c, s);
+    else step32<false>(c, s);
 }
 
 // Largest of the 64 lanes' values, as whole numbers: those of non-negative floats are in the order
@@ -201,89 +242,150 @@ __device__ __forceinline__ void decode(uint32_t qm, uint32_t qv, float sm, float
     }
 }
 
-constexpr uint32_t kInfBits = 0x7F800000u;
+constexpr uint32_t kInfBits = 0x7F800000u, kNanBits = 0x7FC00000u;
 
-__global__ __launch_bounds__(kThreads) void adamw8_kernel(const Chunk* __restrict__ table,
-                                                          Step s) {
-    const Chunk c = table[blockIdx.x];
-    read_hyper(s);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (uint32_t b = wave; b * kBlock < c.n; b += kThreads / 64) {
-        const uint32_t at = b * kBlock + 4 * lane;
-        const int cnt = left(c.n, at);
-        float ps[4], gs[4], ms[4], vs[4];
-        load_float4(c.p, at, cnt, ps);
-        load_grad4(c, at, cnt, gs);
-        decode(load_codes4(c.m, at, cnt), load_codes4(c.v, at, cnt), c.scales[2 * b],
-               c.scales[2 * b + 1], ms, vs);
-        uint32_t am = 0, av = 0;
+// The codes of four elements, as the rounded operations of their definition give them. Those cost
+// some 30 instructions an element for the correctly rounded quotients and roots, more than the
+// memory leaves time for, and matter only where 127*sqrt(.) or 255*sqrt(sqrt(.)) lies next to a
+// half. So the hardware's reciprocal and roots (1 ulp) come first: with them a value is off by at
+// most 4 * 2^-23 of itself from the defined one (reciprocal and product under the root, root, last
+// product, on both sides): 127 * 2^-21 < 2^-14 and 255 * 2^-21 < 2^-13. Lanes that come within twice
+// that of a half take the definition, and so does a block whose scale's reciprocal is not a normal
+// number. Quotients below 2^-96 give 0 either way.
+__device__ __forceinline__ void encode(const float (&m)[4], const float (&v)[4], float sm,
+                                       float sv, uint32_t& qm, uint32_t& qv) {
+    const float om = sm > 0.f ? sm : 1.f, ov = sv > 0.f ? sv : 1.f;
+    const float im = fast_rcp(om), iv = fast_rcp(ov);
+    float tm[4], tv[4];
+    constexpr float kLow = 0x1p-120f, kHigh = 0x1p120f;
+    bool exact = om < kLow || om > kHigh || ov < kLow || ov > kHigh;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float a = __builtin_amdgcn_sqrtf(fabsf(m[i]) * im) * 127.f;
+        const float b = __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(v[i] * iv)) * 255.f;
+        tm[i] = rintf(a);
+        tv[i] = rintf(b);
+        exact |= fabsf(a - tm[i]) > 0.5f - 0x1p-13f || fabsf(b - tv[i]) > 0.5f - 0x1p-12f;
+    }
+    if (exact) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            update(s, gs[i], ps[i], ms[i], vs[i]);
-            if (i < cnt) {
-                am = max(am, __float_as_uint(fabsf(ms[i])));
-                av = max(av, __float_as_uint(fabsf(vs[i])));
-            }
+            tm[i] = rintf(sqrtf(fabsf(m[i]) / om) * 127.f);
+            tv[i] = rintf(sqrtf(sqrtf(v[i] / ov)) * 255.f);
         }
-        am = wave_max(am);
-        av = wave_max(av);
-        const float sm = __uint_as_float(am), sv = __uint_as_float(av);
-        const float om = am ? sm : 1.f, ov = av ? sv : 1.f;
-        uint32_t qm = 0, qv = 0;
+    }
+    qm = qv = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float a = rintf(sqrtf(fabsf(ms[i]) / om) * 127.f);
-            float q = rintf(sqrtf(sqrtf(vs[i] / ov)) * 255.f);
-            if (vs[i] > 0.f) q = fmaxf(q, 1.f);
-            qm |= ((uint32_t)(int)(ms[i] < 0.f ? -a : a) & 255u) << (8 * i);
-            qv |= ((uint32_t)(int)q & 255u) << (8 * i);
-        }
-        if (am >= kInfBits) qm = 0;
-        if (av >= kInfBits) qv = 0;
-        store_float4(c.p, at, cnt, ps);
-        store_codes4(c.m, at, cnt, qm);
-        store_codes4(c.v, at, cnt, qv);
-        if (lane == 0) {
-            c.scales[2 * b] = am >= kInfBits ? __builtin_nanf("") : sm;
-            c.scales[2 * b + 1] = av >= kInfBits ? __builtin_nanf("") : sv;
-        }
-        if (c.copy_type) store_copy4(c, at, cnt, ps);
+    for (int i = 0; i < 4; ++i) {
+        const float q = v[i] > 0.f ? fmaxf(tv[i], 1.f) : tv[i];
+        qm |= ((uint32_t)(int)(m[i] < 0.f ? -tm[i] : tm[i]) & 255u) << (8 * i);
+        qv |= ((uint32_t)(int)q & 255u) << (8 * i);
     }
 }
 
+// A wave takes a block of 256 elements, four a lane.
+template <bool FULL>
+__device__ __forceinline__ void step8(const Chunk& c, const Step& s) {
+    const int lane = threadIdx.x & 63;
+    const uint32_t b = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (!FULL && b * kBlock >= c.n) return;
+    const uint32_t at = b * kBlock + 4 * lane;
+    const auto scales = global<float>(c.scales) + 2 * b;
+    float ps[4], gs[4], ms[4], vs[4];
+    const uint32_t qm0 = load_codes4<FULL>(c.m, at, c.n), qv0 = load_codes4<FULL>(c.v, at, c.n);
+    const float sm0 = scales[0], sv0 = scales[1];
+    load_float4<FULL>(c.p, at, c.n, ps);
+    load_grad4<FULL>(c, at, c.n, gs);
+    decode(qm0, qv0, sm0, sv0, ms, vs);
+    uint32_t am = 0, av = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        update(s, gs[i], ps[i], ms[i], vs[i]);
+        if (FULL || at + i < c.n) {
+            am = max(am, __float_as_uint(fabsf(ms[i])));
+            av = max(av, __float_as_uint(fabsf(vs[i])));
+        }
+    }
+    am = wave_max(am);
+    av = wave_max(av);
+    uint32_t qm, qv;
+    encode(ms, vs, __uint_as_float(am), __uint_as_float(av), qm, qv);
+    if (am >= kInfBits) qm = 0, am = kNanBits;
+    if (av >= kInfBits) qv = 0, av = kNanBits;
+    store_float4<FULL>(c.p, at, c.n, ps);
+    store_codes4<FULL>(c.m, at, c.n, qm);
+    store_codes4<FULL>(c.v, at, c.n, qv);
+    if (lane == 0) {
+        scales[0] = __uint_as_float(am);
+        scales[1] = __uint_as_float(av);
+    }
+    if (c.copy_type) store_copy4<FULL>(c, at, c.n, ps);
+}
+
+__global__ __launch_bounds__(kThreads) void adamw8_kernel(const Chunk* __restrict__ table,
+                                                          Step s) {
+    const Chunk c = load_chunk(table);
+    read_hyper(s);
+    if (c.n == kChunk) step8<true>(c, s);
+    else step8<false>(c, s);
+}
+
 // The float32 states in flat buffers where every tensor begins at a multiple of 256 elements, with
-// zeros up to the next one.
-template <int BITS>
-__global__ __launch_bounds__(kThreads) void adamw_states_kernel(const Chunk* __restrict__ table,
-                                                                float* __restrict__ m,
-                                                                float* __restrict__ v) {
-    const Chunk c = table[blockIdx.x];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (uint32_t b = wave; b * kBlock < c.n; b += kThreads / 64) {
-        const uint32_t at = b * kBlock + 4 * lane;
-        const int cnt = left(c.n, at);
-        float ms[4], vs[4];
+// zeros up to the next one: a wave takes two of a chunk's blocks of 256 elements (48 Evoformer
+// blocks' step and states: 410 us, with one or four blocks a wave 417 and 421).
+constexpr int WB = 2;
+template <int BITS, bool FULL>
+__device__ __forceinline__ void states(const Chunk& c, float* m, float* v) {
+    const int lane = threadIdx.x & 63;
+    const uint32_t b0 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * WB;
+    float ms[WB][4], vs[WB][4], sm[WB], sv[WB];
+    uint32_t qm[WB], qv[WB];
+#pragma unroll
+    for (int k = 0; k < WB; ++k) {
+        const uint32_t b = b0 + k, at = b * kBlock + 4 * lane;
         if (BITS == 8) {
-            decode(load_codes4(c.m, at, cnt), load_codes4(c.v, at, cnt), c.scales[2 * b],
-                   c.scales[2 * b + 1], ms, vs);
+            const auto scales = global<const float>(c.scales);
+            const bool there = FULL || b * kBlock < c.n;
+            qm[k] = load_codes4<FULL>(c.m, at, c.n);
+            qv[k] = load_codes4<FULL>(c.v, at, c.n);
+            sm[k] = there ? scales[2 * b] : 0.f;
+            sv[k] = there ? scales[2 * b + 1] : 0.f;
+        } else {
+            load_float4<FULL>(c.m, at, c.n, ms[k]);
+            load_float4<FULL>(c.v, at, c.n, vs[k]);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < WB; ++k) {
+        const uint32_t b = b0 + k, at = b * kBlock + 4 * lane;
+        if (!FULL && b * kBlock >= c.n) break;
+        if (BITS == 8) {
+            decode(qm[k], qv[k], sm[k], sv[k], ms[k], vs[k]);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (i >= cnt) ms[i] = vs[i] = 0.f;  // a NaN scale's as well
-        } else {
-            load_float4(static_cast<const float*>(c.m), at, cnt, ms);
-            load_float4(static_cast<const float*>(c.v), at, cnt, vs);
+                if (!FULL && at + i >= c.n) ms[k][i] = vs[k][i] = 0.f;  // a NaN scale's as well
         }
-        *reinterpret_cast<f32x4*>(m + c.at + at) = f32x4{ms[0], ms[1], ms[2], ms[3]};
-        *reinterpret_cast<f32x4*>(v + c.at + at) = f32x4{vs[0], vs[1], vs[2], vs[3]};
+        __builtin_nontemporal_store(f32x4{ms[k][0], ms[k][1], ms[k][2], ms[k][3]},
+                                    reinterpret_cast<f32x4*>(m + c.at + at));
+        __builtin_nontemporal_store(f32x4{vs[k][0], vs[k][1], vs[k][2], vs[k][3]},
+                                    reinterpret_cast<f32x4*>(v + c.at + at));
     }
+}
+constexpr int kStatesThreads = kChunk / 4 / WB;
+template <int BITS>
+__global__ __launch_bounds__(kStatesThreads) void adamw_states_kernel(
+    const Chunk* __restrict__ table, float* __restrict__ m, float* __restrict__ v) {
+    const Chunk c = load_chunk(table);
+    if (c.n == kChunk) states<BITS, true>(c, m, v);
+    else states<BITS, false>(c, m, v);
 }
 
 // ---------------------------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------------------------
 
-// Elements a chunk: few enough that a small parameter set still fills the chip.
-constexpr int64_t kSmallChunk = 1024, kLargeChunk = 4096;
+// A launch holds fewer than 2^32 threads.
+constexpr int64_t kMaxChunks = (1 << 24) - 1;
 
 struct Span {
     uintptr_t beg, end;
@@ -329,15 +431,14 @@ bool overlapping(std::vector<Span>& spans) {
 
 clk_status build_table(const char* who, const clk_adamw_tensor* tensors, int64_t n, int bits,
                        void* table, size_t table_bytes, int64_t* chunks) {
-    int64_t total = 0, large = 0, small = 0;
+    int64_t total = 0, count = 0;
     std::vector<Span> spans;
     for (int64_t i = 0; i < n; ++i) {
         const clk_adamw_tensor& t = tensors[i];
         const clk_status s = check_tensor(who, t, i, bits);
         if (s != CLK_OK) return s;
         total += t.numel;
-        large += up(t.numel, kLargeChunk);
-        small += up(t.numel, kSmallChunk);
+        count += up(t.numel, kChunk);
         const auto span = [&](const void* p, int64_t bytes, bool written) {
             const uintptr_t b = reinterpret_cast<uintptr_t>(p);
             if (p && bytes > 0) spans.push_back({b, b + (uintptr_t)bytes, written});
@@ -353,9 +454,7 @@ clk_status build_table(const char* who, const clk_adamw_tensor* tensors, int64_t
     if (overlapping(spans))
         return fail(CLK_INVALID_ARGUMENT,
                     "%s: tensors overlap (parameters, states, scales and copies are written)", who);
-    const int64_t chunk = large < 2048 ? kSmallChunk : kLargeChunk;
-    const int64_t count = chunk == kSmallChunk ? small : large;
-    if (count >= (1 << 24))
+    if (count > kMaxChunks)
         return fail(CLK_INVALID_ARGUMENT, "%s: %lld elements are too many", who, (long long)total);
     *chunks = count;
     if (!table) return ok();
@@ -366,7 +465,7 @@ clk_status build_table(const char* who, const clk_adamw_tensor* tensors, int64_t
     int64_t base = 0;
     for (int64_t i = 0; i < n; ++i) {
         const clk_adamw_tensor& t = tensors[i];
-        for (int64_t o = 0; o < t.numel; o += chunk) {
+        for (int64_t o = 0; o < t.numel; o += kChunk) {
             Chunk c;
             c.p = t.param + o;
             c.g = static_cast<const char*>(t.grad) + o * (int64_t)elem_size(t.grad_dtype);
@@ -375,7 +474,7 @@ clk_status build_table(const char* who, const clk_adamw_tensor* tensors, int64_t
             c.scales = bits == 8 ? t.scales + 2 * (o / kBlock) : nullptr;
             c.copy = t.copy ? static_cast<char*>(t.copy) + 2 * o : nullptr;
             c.at = base + o;
-            c.n = (uint32_t)std::min(chunk, t.numel - o);
+            c.n = (uint32_t)std::min<int64_t>(kChunk, t.numel - o);
             c.grad_type = (uint16_t)t.grad_dtype;
             c.copy_type = t.copy ? (uint16_t)t.copy_dtype : 0;
             std::memcpy(to, &c, sizeof(c));
@@ -389,7 +488,7 @@ clk_status build_table(const char* who, const clk_adamw_tensor* tensors, int64_t
 clk_status check_call(const char* who, const void* table, int64_t chunks, int bits) {
     if (bits != 8 && bits != 32)
         return fail(CLK_INVALID_ARGUMENT, "%s: states of %d bits (8, 32)", who, bits);
-    if (chunks < 0 || chunks >= (1 << 24))
+    if (chunks < 0 || chunks > kMaxChunks)
         return fail(CLK_INVALID_ARGUMENT, "%s: %lld chunks", who, (long long)chunks);
     if (chunks > 0 && (!table || !aligned16(table)))
         return fail(CLK_INVALID_ARGUMENT, "%s: the table must be a 16-byte aligned device pointer",
@@ -425,8 +524,9 @@ extern "C" clk_status clk_adamw_step(hipStream_t stream, const void* table, int6
     if (s != CLK_OK) return s;
     if (!(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0))
         return fail(CLK_INVALID_ARGUMENT, "%s: betas must lie in [0, 1)", who);
-    if (!((float)eps > 0.f) || !std::isfinite(eps))
-        return fail(CLK_INVALID_ARGUMENT, "%s: eps must be positive and finite", who);
+    if (!((float)eps >= 0x1p-126f) || !std::isfinite((float)eps))
+        return fail(CLK_INVALID_ARGUMENT, "%s: eps must be positive (a normal float32) and finite",
+                    who);
     if (!std::isfinite(weight_decay))
         return fail(CLK_INVALID_ARGUMENT, "%s: weight_decay must be finite", who);
     if (hyper) {
@@ -472,8 +572,8 @@ extern "C" clk_status clk_adamw_states(hipStream_t stream, const void* table, in
     const Chunk* t = static_cast<const Chunk*>(table);
     KernelTimer timer("adamw_states", stream);
     if (state_bits == 8)
-        adamw_states_kernel<8><<<(int)chunks, kThreads, 0, stream>>>(t, exp_avg, exp_avg_sq);
+        adamw_states_kernel<8><<<(int)chunks, kStatesThreads, 0, stream>>>(t, exp_avg, exp_avg_sq);
     else
-        adamw_states_kernel<32><<<(int)chunks, kThreads, 0, stream>>>(t, exp_avg, exp_avg_sq);
+        adamw_states_kernel<32><<<(int)chunks, kStatesThreads, 0, stream>>>(t, exp_avg, exp_avg_sq);
     return check_launch(who);
 }
