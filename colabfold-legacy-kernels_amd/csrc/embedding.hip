@@ -61,7 +61,10 @@ __global__ __launch_bounds__(kThreads) void embed_kernel(
 }
 
 // ---------------------------------------------------------------------------------------------
-// Sorting the tokens: keys are rows of the table, V for an absent token (they come last).
+// Sorting the tokens: keys are rows of the table, V for an absent token (they come last). These
+// kernels wait for memory more than they use it: blocks behind the ones that sort set the gradient
+// to zero meanwhile, a part in each kernel, so that the sums write only the rows that tokens name
+// (16,411 tokens of 30,011 rows of 640 columns: all of it in the first kernel 48 us, in parts 43).
 // ---------------------------------------------------------------------------------------------
 template <typename ID>
 __device__ __forceinline__ uint32_t token_key(const ID* ids, int64_t i, uint32_t V) {
@@ -69,16 +72,44 @@ __device__ __forceinline__ uint32_t token_key(const ID* ids, int64_t i, uint32_t
     return id >= 0 && id < (int64_t)V ? (uint32_t)id : V;
 }
 
-// Few tokens: each one's place is the number of tokens before it, counted over all of them. M^2
-// comparisons over the whole chip, in one launch: 16 tokens a block, 16 threads a token.
-constexpr int kRankMax = 8192;  // 32 KB of keys in LDS
+// Keeps a wave's LDS operations in the order of the program (the hardware does not reorder them).
+__device__ __forceinline__ void wave_order() {
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_wave_barrier();
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+}
+
+// A part of the gradient, floats [beg, end) with beg a multiple of four, that blocks first ..
+// first + blocks - 1 of a grid fill.
+struct Zero {
+    float* p;
+    size_t beg, end;
+    int first, blocks;
+};
+// True for a block that fills (and has filled).
+__device__ __forceinline__ bool zero_block(const Zero& z) {
+    if ((int)blockIdx.x < z.first) return false;
+    const size_t end4 = z.end / 4, step = (size_t)z.blocks * kThreads;
+    const size_t b = (size_t)((int)blockIdx.x - z.first);
+    f32x4* p4 = reinterpret_cast<f32x4*>(z.p);
+    for (size_t i = z.beg / 4 + b * kThreads + threadIdx.x; i < end4; i += step)
+        __builtin_nontemporal_store(f32x4{0.f, 0.f, 0.f, 0.f}, p4 + i);
+    if (b == 0 && threadIdx.x < z.end % 4) z.p[4 * end4 + threadIdx.x] = 0.f;
+    return true;
+}
+
+// Up to kRankMax tokens: each one's place is the number of tokens before it, counted over all of
+// them. M^2 comparisons over the whole chip, in one launch: 16 tokens a block, 16 threads a token.
+constexpr int kRankMax = 4096;  // 12 us, as two digits' passes; 8192 tokens 21 us against 16
 constexpr int kRankTokens = 16, kRankSlices = kThreads / kRankTokens;
 template <typename ID>
 __global__ __launch_bounds__(kThreads) void embed_rank_kernel(const ID* __restrict__ ids, int M,
                                                               uint32_t V,
                                                               uint32_t* __restrict__ keys,
-                                                              uint32_t* __restrict__ order) {
+                                                              uint32_t* __restrict__ order,
+                                                              Zero zero) {
     __shared__ __attribute__((aligned(16))) uint32_t k[kRankMax];
+    if (zero_block(zero)) return;
     const int padded = (M + 3) & ~3;
     for (int i = threadIdx.x; i < padded; i += kThreads)
         k[i] = i < M ? token_key(ids, i, V) : ~0u;  // past every token
@@ -100,10 +131,20 @@ __global__ __launch_bounds__(kThreads) void embed_rank_kernel(const ID* __restri
     }
 }
 
-// More tokens: a stable least-significant-digit radix sort, 8 bits a pass. A tile is 2048 tokens;
-// counts[digit][tile] is summed over the tiles of each digit (one block a digit), and the scatter
-// adds the digits before.
-constexpr int kTile = 2048, kDigits = 256;
+// More tokens: a stable least-significant-digit radix sort, 8 bits a pass: the digits of each tile of
+// tokens are counted, the counts summed over the tiles before, and the tokens moved. Up to
+// kFewTiles tiles the moving blocks sum the counts themselves; more are summed by a kernel of its
+// own, a block a digit. Count (digit, tile) is at digit * by_digit + tile * by_tile.
+constexpr int kTile = 1024, kDigits = 256;
+constexpr int64_t kFewTiles = 32;  // at 128 tiles the move takes 12 us, after a scan 8 + 2
+struct Counts {
+    uint32_t* n;
+    int64_t tiles;
+    size_t by_digit, by_tile;
+    __device__ __forceinline__ uint32_t& at(int digit, int64_t tile) const {
+        return n[digit * by_digit + tile * by_tile];
+    }
+};
 
 template <typename ID>
 struct FirstKeys {  // the first pass reads the ids themselves
@@ -120,9 +161,9 @@ struct NextKeys {
 
 template <typename SRC>
 __global__ __launch_bounds__(kThreads) void embed_count_kernel(SRC src, int64_t M, int shift,
-                                                               int64_t tiles,
-                                                               uint32_t* __restrict__ counts) {
+                                                               Counts counts, Zero zero) {
     __shared__ uint32_t n[kDigits];
+    if (zero_block(zero)) return;
     n[threadIdx.x] = 0;
     __syncthreads();
     const int64_t base = (int64_t)blockIdx.x * kTile;
@@ -132,20 +173,18 @@ __global__ __launch_bounds__(kThreads) void embed_count_kernel(SRC src, int64_t 
         if (i < M) atomicAdd(&n[(src.key(i) >> shift) & 255u], 1u);  // whole numbers: any order
     }
     __syncthreads();
-    counts[(size_t)threadIdx.x * tiles + blockIdx.x] = n[threadIdx.x];
+    counts.at(threadIdx.x, blockIdx.x) = n[threadIdx.x];
 }
 
 // Exclusive sums of one digit's counts over the tiles, in place, and its total.
-__global__ __launch_bounds__(kThreads) void embed_scan_kernel(uint32_t* __restrict__ counts,
-                                                              int64_t tiles,
+__global__ __launch_bounds__(kThreads) void embed_scan_kernel(Counts counts,
                                                               uint32_t* __restrict__ totals) {
     __shared__ uint32_t wave_sum[kThreads / 64];
-    uint32_t* row = counts + (size_t)blockIdx.x * tiles;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     uint32_t carry = 0;
-    for (int64_t t0 = 0; t0 < tiles; t0 += kThreads) {
+    for (int64_t t0 = 0; t0 < counts.tiles; t0 += kThreads) {
         const int64_t t = t0 + threadIdx.x;
-        const uint32_t own = t < tiles ? row[t] : 0;
+        const uint32_t own = t < counts.tiles ? counts.at(blockIdx.x, t) : 0;
         uint32_t sum = own;
 #pragma unroll
         for (int s = 1; s < 64; s <<= 1) {
@@ -160,7 +199,7 @@ __global__ __launch_bounds__(kThreads) void embed_scan_kernel(uint32_t* __restri
             if (w < wave) before += wave_sum[w];
             all += wave_sum[w];
         }
-        if (t < tiles) row[t] = before + sum - own;
+        if (t < counts.tiles) counts.at(blockIdx.x, t) = before + sum - own;
         carry += all;
         __syncthreads();
     }
@@ -169,20 +208,38 @@ __global__ __launch_bounds__(kThreads) void embed_scan_kernel(uint32_t* __restri
 
 // Moves a tile's tokens to their places. Wave w takes the tile's w-th quarter, 64 consecutive
 // tokens a round; lanes with equal digits find each other by eight ballots, so a token's rank
-// follows the order of the tokens.
+// follows the order of the tokens. `totals`: the scan kernel's, or null.
 template <typename SRC>
 __global__ __launch_bounds__(kThreads) void embed_scatter_kernel(
-    SRC src, int64_t M, int shift, int64_t tiles, const uint32_t* __restrict__ counts,
-    const uint32_t* __restrict__ totals, uint32_t* __restrict__ keys,
-    uint32_t* __restrict__ order) {
+    SRC src, int64_t M, int shift, Counts counts, const uint32_t* __restrict__ totals,
+    uint32_t* __restrict__ keys, uint32_t* __restrict__ order, Zero zero) {
     constexpr int kWaves = kThreads / 64, kRounds = kTile / kThreads;
     __shared__ uint32_t n[kWaves][kDigits];
     __shared__ uint32_t wave_sum[kWaves];
+    if (zero_block(zero)) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) n[w][threadIdx.x] = 0;
-    // Exclusive sum of the digits' totals (one thread a digit).
-    const uint32_t own = totals[threadIdx.x];
+    // One thread a digit: its tokens in the tiles before this one, and in all.
+    uint32_t earlier = 0, own = 0;
+    if (totals) {
+        earlier = counts.at(threadIdx.x, blockIdx.x);
+        own = totals[threadIdx.x];
+    } else {
+        constexpr int U = 16;
+        for (int t0 = 0; t0 < (int)counts.tiles; t0 += U) {
+            uint32_t k[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                k[u] = t0 + u < (int)counts.tiles ? counts.at(threadIdx.x, t0 + u) : 0;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                own += k[u];
+                earlier += t0 + u < (int)blockIdx.x ? k[u] : 0;
+            }
+        }
+    }
+    // Exclusive sum of the digits' totals.
     uint32_t sum = own;
 #pragma unroll
     for (int s = 1; s < 64; s <<= 1) {
@@ -191,9 +248,8 @@ __global__ __launch_bounds__(kThreads) void embed_scatter_kernel(
     }
     if (lane == 63) wave_sum[wave] = sum;
     __syncthreads();
-    uint32_t first = sum - own;
+    uint32_t first = sum - own + earlier;
     for (int w = 0; w < wave; ++w) first += wave_sum[w];
-    first += counts[(size_t)threadIdx.x * tiles + blockIdx.x];
 
     const int64_t base = (int64_t)blockIdx.x * kTile + wave * (kTile / kWaves);
     uint32_t key[kRounds], rank[kRounds];
@@ -218,10 +274,10 @@ __global__ __launch_bounds__(kThreads) void embed_scatter_kernel(
             // each digit writes the new count.
             const uint32_t had = n[wave][digit];
             rank[u] = had + (uint32_t)__popcll(below);
-            __builtin_amdgcn_wave_barrier();
+            wave_order();
             if (below == 0) n[wave][digit] = had + (uint32_t)__popcll(same);
         }
-        __builtin_amdgcn_wave_barrier();
+        wave_order();
     }
     __syncthreads();
     // Where each wave's tokens of a digit begin.
@@ -244,54 +300,51 @@ __global__ __launch_bounds__(kThreads) void embed_scatter_kernel(
 }
 
 // ---------------------------------------------------------------------------------------------
-// Sums of the sorted tokens. The sorted order is cut into chunks of kChunk tokens. A group of
-// LPR lanes takes one chunk and one slice of LPR vectors of the columns, keeps the running sum in
-// registers and stores it where the row ends: into the table if the run also began in the chunk,
-// else into a partial of the chunk: `tail` for a run that begins here and goes on, `head` for one
-// that began before (whether or not it goes on).
+// Sums of the sorted tokens. A group of LPR lanes takes kRun tokens of the sorted order and one
+// slice of LPR vectors of the columns; it keeps the running sum in registers and stores it where
+// the row ends: into the table if the run also began in the group, else in LDS, as the group's
+// `head` (of a run that began before it). A group whose last run goes on then adds the heads of the
+// groups that it goes on into; what the block's ends cut leaves as a head or a tail of the block's
+// chunk of tokens, and embed_join_kernel joins those.
 // ---------------------------------------------------------------------------------------------
-constexpr int kChunk = 32;
-
-// First position of the sorted keys that is not below `key`.
-__device__ __forceinline__ uint32_t lower_bound(const uint32_t* keys, uint32_t M, uint32_t key) {
-    uint32_t lo = 0, n = M;
-    while (n > 0) {
-        const uint32_t half = n / 2;
-        if (keys[lo + half] < key) {
-            lo += half + 1;
-            n -= half + 1;
-        } else {
-            n = half;
-        }
-    }
-    return lo;
+constexpr int kRun = 16;
+template <int LPR>
+constexpr int chunk_tokens() {
+    return kThreads / LPR * kRun;
 }
 
-// Blocks [0, sum_blocks) sum; the others write starts[v] = first sorted token of row v, v <= V.
 template <typename TR, int LPR, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void embed_sum_kernel(
     const typename TR::elem* __restrict__ dout, const uint32_t* __restrict__ keys,
     const uint32_t* __restrict__ order, float* __restrict__ dtable, float* __restrict__ head,
-    float* __restrict__ tail, uint32_t* __restrict__ starts, uint32_t M, uint32_t V, int C,
-    uint32_t chunks, FastDiv slices, uint32_t sum_blocks, float scale) {
-    constexpr int N = Vec<TR>::N, U = 8;
-    static_assert(kChunk % U == 0);
-    if (blockIdx.x >= sum_blocks) {
-        const uint32_t v = (blockIdx.x - sum_blocks) * kThreads + threadIdx.x;
-        if (v <= V) starts[v] = lower_bound(keys, M, v);
-        return;
-    }
-    const uint32_t group = blockIdx.x * (kThreads / LPR) + threadIdx.x / LPR;
-    const uint32_t chunk = div_by(group, slices), slice = group - chunk * slices.d;
-    if (chunk >= chunks) return;
-    const int col = (int)(slice * LPR + threadIdx.x % LPR) * N;
-    if (col >= C) return;
-    const uint32_t beg = chunk * kChunk, end = M - beg < kChunk ? M : beg + kChunk;
-    uint32_t cur = keys[beg];
-    bool began = beg == 0 || keys[beg - 1] != cur;  // the current run began in this chunk
+    float* __restrict__ tail, uint32_t M, uint32_t V, int C, FastDiv slices, float scale) {
+    constexpr int N = Vec<TR>::N, U = 8, G = kThreads / LPR, W = LPR * N;
+    static_assert(kRun % U == 0);
+    __shared__ __attribute__((aligned(16))) float heads[G][W];
+    __shared__ uint32_t first_key[G];
+    const uint32_t chunk = div_by(blockIdx.x, slices), slice = blockIdx.x - chunk * slices.d;
+    const int g = threadIdx.x / LPR, s = threadIdx.x % LPR;
+    const int col = (int)(slice * LPR + s) * N;
+    const bool cols = col < C;
+    const uint32_t beg = chunk * chunk_tokens<LPR>() + g * kRun;
+    const uint32_t end = beg >= M ? beg : M - beg < kRun ? M : beg + kRun;
+    uint32_t cur = beg < M ? keys[beg] : V;
+    if (s == 0) first_key[g] = cur;
+    // A head run began before the group; the last run goes on behind it.
+    const bool has_head = beg > 0 && beg < M && cur < V && keys[beg - 1] == cur;
+    bool began = !has_head, has_tail = false;
     float acc[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) acc[i] = 0.f;
+    const auto keep = [&](float (&piece)[W]) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) piece[s * N + i] = acc[i];
+    };
+    const auto finish = [&](uint32_t row) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] *= scale;
+        if (cols) store_floats(dtable + (size_t)row * C, col, C, acc);
+    };
     for (uint32_t i0 = beg; i0 < end && cur < V; i0 += U) {
         uint32_t k[U], at[U];
 #pragma unroll
@@ -302,19 +355,14 @@ __global__ __launch_bounds__(kThreads) void embed_sum_kernel(
         u32x4 raw[U];
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            raw[u] = k[u] < V ? load_vec<TR, WHOLE>(dout + (size_t)at[u] * C, col, C)
-                              : u32x4{0u, 0u, 0u, 0u};
+            raw[u] = k[u] < V && cols ? load_vec<TR, WHOLE>(dout + (size_t)at[u] * C, col, C)
+                                      : u32x4{0u, 0u, 0u, 0u};
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (i0 + u >= end) break;
             if (k[u] != cur) {
-                if (began) {
-#pragma unroll
-                    for (int i = 0; i < N; ++i) acc[i] *= scale;
-                    store_floats(dtable + (size_t)cur * C, col, C, acc);
-                } else {
-                    store_floats(head + (size_t)chunk * C, col, C, acc);
-                }
+                if (began) finish(cur);
+                else keep(heads[g]);
 #pragma unroll
                 for (int i = 0; i < N; ++i) acc[i] = 0.f;
                 cur = k[u];
@@ -327,108 +375,86 @@ __global__ __launch_bounds__(kThreads) void embed_sum_kernel(
             for (int i = 0; i < N; ++i) acc[i] += v[i];
         }
     }
-    if (cur >= V) return;
-    if (!began) {
-        store_floats(head + (size_t)chunk * C, col, C, acc);
-    } else if (end < M && keys[end] == cur) {
-        store_floats(tail + (size_t)chunk * C, col, C, acc);
-    } else {
+    if (cur < V) {
+        if (!began) {
+            keep(heads[g]);
+        } else if (end < M && keys[end] == cur) {
+            has_tail = true;
+        } else {
+            finish(cur);
+        }
+    }
+    __syncthreads();
+    // The run of a tail goes on through the groups that begin with its key; the first group's head
+    // is the block's.
+    if (!has_tail && !(g == 0 && has_head)) return;
+    for (int own = 0; own < 2; ++own) {
+        if (own == 0 ? !(g == 0 && has_head) : !has_tail) continue;
+        const uint32_t key = own == 0 ? first_key[0] : cur;
+        int j = g + own;
+        float sum[N];
 #pragma unroll
-        for (int i = 0; i < N; ++i) acc[i] *= scale;
-        store_floats(dtable + (size_t)cur * C, col, C, acc);
+        for (int i = 0; i < N; ++i) sum[i] = own == 0 ? 0.f : acc[i];
+        for (; j < G && first_key[j] == key; ++j)
+#pragma unroll
+            for (int i = 0; i < N; ++i) sum[i] += heads[j][s * N + i];
+        const uint32_t after = (chunk + 1) * chunk_tokens<LPR>();
+        float* to = head + (size_t)chunk * C;
+        if (own == 1) {
+            const bool goes_on = j == G && after < M && keys[after] == key;
+            to = goes_on ? tail + (size_t)chunk * C : dtable + (size_t)key * C;
+#pragma unroll
+            for (int i = 0; i < N; ++i) sum[i] *= goes_on ? 1.f : scale;
+        }
+        if (cols) store_floats(to, col, C, sum);
     }
 }
 
-// Runs cut by chunk ends: tail of their first chunk plus the heads of the others. A run over at
-// most kLongRun chunks is joined by one wave, with the rows that no token named set to zero; a
-// longer one by a block of its own.
-constexpr int kLongRun = 64;
-struct Run {
-    uint32_t first, last;  // chunks
-    bool none;
-};
-__device__ __forceinline__ Run run_of(const uint32_t* starts, uint32_t v) {
-    const uint32_t s = starts[v], e = starts[v + 1];
-    return Run{s / kChunk, (e - 1) / kChunk, s == e};
-}
-
-__device__ __forceinline__ f32x4 load4(const float* p, int col, int C) {
-    float v[4];
-    load_floats<4, false>(p, col, C, 0.f, v);
-    return f32x4{v[0], v[1], v[2], v[3]};
-}
-
+// Runs cut by the ends of chunks: the tail of the chunk they begin in plus the heads of the chunks
+// they go on into, whose first keys are theirs. A block looks at one chunk and 256 columns, its
+// waves take the heads in turn.
 __global__ __launch_bounds__(kThreads) void embed_join_kernel(
-    const float* __restrict__ head, const float* __restrict__ tail,
-    const uint32_t* __restrict__ starts, float* __restrict__ dtable, uint32_t V, int C,
-    FastDiv slices, float scale) {
-    const uint32_t items = V * slices.d, step = gridDim.x * (kThreads / 64);
-    for (uint32_t item = blockIdx.x * (kThreads / 64) + threadIdx.x / 64; item < items;
-         item += step) {
-        const uint32_t v = div_by(item, slices);
-        const int col = (int)((item - v * slices.d) * 64 + threadIdx.x % 64) * 4;
-        if (col >= C) continue;
-        const Run run = run_of(starts, v);
-        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-        if (!run.none) {
-            if (run.first == run.last || run.last - run.first >= kLongRun) continue;
-            sum = load4(tail + (size_t)run.first * C, col, C);
-            constexpr int U = 8;
-            for (uint32_t c0 = run.first + 1; c0 <= run.last; c0 += U) {
-                f32x4 p[U];
-#pragma unroll
-                for (int u = 0; u < U; ++u)
-                    p[u] = c0 + u <= run.last ? load4(head + (size_t)(c0 + u) * C, col, C)
-                                              : f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int u = 0; u < U; ++u) sum += p[u];
-            }
-            sum *= scale;
-        }
-        const float v4[4] = {sum[0], sum[1], sum[2], sum[3]};
-        store_floats(dtable + (size_t)v * C, col, C, v4);
-    }
-}
-
-// A run over more than kLongRun chunks holds a multiple of kLongRun after its first chunk: block
-// b looks at chunk b * kLongRun, and the first one of a run sums it, 16 waves taking its chunks in
-// turn.
-constexpr int kLongWaves = 16;
-__global__ __launch_bounds__(64 * kLongWaves) void embed_join_long_kernel(
     const uint32_t* __restrict__ keys, const float* __restrict__ head,
-    const float* __restrict__ tail, const uint32_t* __restrict__ starts,
-    float* __restrict__ dtable, uint32_t V, int C, float scale) {
-    __shared__ f32x4 part[kLongWaves][64];
-    const uint32_t at = (blockIdx.x + 1) * kLongRun;
-    const uint32_t v = keys[(size_t)at * kChunk];
-    if (v >= V) return;
-    const Run run = run_of(starts, v);
-    if (run.last - run.first < kLongRun || at - run.first > kLongRun || at == run.first) return;
+    const float* __restrict__ tail, float* __restrict__ dtable, uint32_t V, int C,
+    uint32_t chunks, int tokens, FastDiv slices, float scale) {
+    constexpr int kWaves = kThreads / 64, U = 16;
+    __shared__ f32x4 part[kWaves][64];
+    const uint32_t c = div_by(blockIdx.x, slices);  // not the last chunk
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int col = (int)(blockIdx.y * 64 + lane) * 4;
+    const int col = (int)((blockIdx.x - c * slices.d) * 64 + lane) * 4;
+    const size_t beg = (size_t)c * tokens;
+    const uint32_t before = keys[c > 0 ? beg - 1 : 0], begins = keys[beg],
+                   ends = keys[beg + tokens - 1], key = keys[beg + tokens];
+    // The run that the next chunk begins with began in this one, and is no absent tokens'.
+    if (key >= V || ends != key || (c > 0 && begins == key && before == key)) return;
+    const auto load = [&](const float* p, uint32_t chunk) {
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+        if (col < C) load_floats<4, false>(p + (size_t)chunk * C, col, C, 0.f, v);
+        return f32x4{v[0], v[1], v[2], v[3]};
+    };
     f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-    if (col < C) {
-        if (wave == 0) sum = load4(tail + (size_t)run.first * C, col, C);
-        constexpr int U = 8;
-        for (uint32_t c0 = run.first + 1 + wave; c0 <= run.last; c0 += U * kLongWaves) {
-            f32x4 p[U];
+    if (wave == 0) sum = load(tail, c);
+    // The heads are loaded along with the keys that say whether they are this run's.
+    for (uint32_t c0 = c + 1 + wave;; c0 += U * kWaves) {
+        f32x4 p[U];
+        uint32_t k[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const uint32_t c = c0 + u * kLongWaves;
-                p[u] = c <= run.last ? load4(head + (size_t)c * C, col, C)
-                                     : f32x4{0.f, 0.f, 0.f, 0.f};
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u) sum += p[u];
+        for (int u = 0; u < U; ++u) {
+            const uint32_t at = c0 + u * kWaves, in = min(at, chunks - 1);
+            k[u] = at < chunks ? keys[(size_t)in * tokens] : V;
+            p[u] = load(head, in);
         }
+#pragma unroll
+        for (int u = 0; u < U; ++u) sum += k[u] == key ? p[u] : f32x4{0.f, 0.f, 0.f, 0.f};
+        if (k[U - 1] != key) break;
     }
     part[wave][lane] = sum;
     __syncthreads();
     if (wave == 0 && col < C) {
-        for (int w = 1; w < kLongWaves; ++w) sum += part[w][lane];
-        sum *= scale;
-        const float v4[4] = {sum[0], sum[1], sum[2], sum[3]};
-        store_floats(dtable + (size_t)v * C, col, C, v4);
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) sum += part[w][lane];
+        const float v4[4] = {sum[0] * scale, sum[1] * scale, sum[2] * scale, sum[3] * scale};
+        store_floats(dtable + (size_t)key * C, col, C, v4);
     }
 }
 
@@ -709,6 +735,10 @@ __global__ __launch_bounds__(kThreads) void embed_zero_kernel(float* __restrict_
 constexpr int64_t kMaxBlocks = 1 << 22;
 size_t pad256(size_t n) { return (n + 255) & ~(size_t)255; }
 
+// Lanes that take a row of nvec vectors in embed_sum_kernel: as many as it has, up to the 16 that
+// read 256 bytes of it.
+int lanes_a_row(int64_t nvec) { return nvec > 8 ? 16 : nvec > 4 ? 8 : nvec > 2 ? 4 : 2; }
+
 // What the gradient keeps in its workspace, as offsets in bytes.
 struct BwdPlan {
     // Tables of few rows: parts of `tokens` tokens, their partial sums `stride` floats apart.
@@ -720,7 +750,7 @@ struct BwdPlan {
     bool ranked;
     int passes;
     int64_t tiles, chunks;
-    size_t keys[2], order[2], counts, totals, starts, head, tail, bytes;
+    size_t keys[2], order[2], counts, totals, head, tail, bytes;
 };
 BwdPlan bwd_plan(int64_t M, int64_t V, int64_t C) {
     BwdPlan p = {};
@@ -740,7 +770,7 @@ BwdPlan bwd_plan(int64_t M, int64_t V, int64_t C) {
     p.passes = 1;
     while ((V >> (8 * p.passes)) != 0) ++p.passes;  // keys are 0 .. V
     p.tiles = up(M, kTile);
-    p.chunks = up(M, kChunk);
+    p.chunks = up(M, kThreads / lanes_a_row(up(C, 4)) * kRun);  // float32 rows have the most
     size_t at = 0;
     const auto take = [&](size_t n) {
         const size_t here = at;
@@ -756,7 +786,6 @@ BwdPlan bwd_plan(int64_t M, int64_t V, int64_t C) {
         p.counts = take((size_t)p.tiles * kDigits * 4);
         p.totals = take(kDigits * 4);
     }
-    p.starts = take((size_t)(V + 1) * 4);
     p.head = take((size_t)p.chunks * C * 4);
     p.tail = take((size_t)p.chunks * C * 4);
     p.bytes = at;
@@ -774,7 +803,7 @@ clk_status validate(const char* who, clk_dtype dtype, clk_dtype ids_dtype, int64
     if (M < 0 || V < 0 || C <= 0)
         return fail(CLK_INVALID_ARGUMENT, "%s: ids [M], table [V,C] with C > 0 expected", who);
     // These keep token, row and chunk numbers in 31 bits and a launch's threads in 32.
-    if (M > (1 << 30) || V > (1 << 30) - 1 || C > (1 << 20) || M * C > ((int64_t)1 << 38) ||
+    if (M > (1 << 30) || V > (1 << 30) - 1 || C > (1 << 20) || M * C > ((int64_t)1 << 37) ||
         V * C > ((int64_t)1 << 37))
         return fail(CLK_INVALID_ARGUMENT, "%s: M=%lld, [V,C] = [%lld,%lld] too large", who,
                     (long long)M, (long long)V, (long long)C);
@@ -799,27 +828,38 @@ void launch_fwd(hipStream_t st, const void* table, const void* ids, void* out, i
 }
 
 template <typename ID>
-void sort_tokens(hipStream_t st, const ID* ids, char* ws, const BwdPlan& p, int64_t M, int64_t V,
-                 uint32_t** keys, uint32_t** order) {
+void sort_tokens(hipStream_t st, const ID* ids, float* dtable, char* ws, const BwdPlan& p,
+                 int64_t M, int64_t V, int64_t C, uint32_t** keys, uint32_t** order) {
     const auto at = [&](size_t off) { return reinterpret_cast<uint32_t*>(ws + off); };
+    // Part k of the zeros, behind `first` other blocks: 16 KB a block, up to 8192 blocks.
+    const size_t n = (size_t)V * C;
+    const int parts = p.ranked ? 1 : 2 * p.passes;
+    const auto zero = [&](int k, int64_t first) {
+        const size_t beg = n / 4 * k / parts * 4, end = k + 1 == parts ? n : n / 4 * (k + 1) / parts * 4;
+        return Zero{dtable, beg, end, (int)first, (int)std::min<int64_t>(up(end - beg, 4096), 8192)};
+    };
+    *keys = at(p.keys[0]);
+    *order = at(p.order[0]);
     if (p.ranked) {
-        *keys = at(p.keys[0]);
-        *order = at(p.order[0]);
+        const Zero z = zero(0, up(M, kRankTokens));
         KernelTimer timer("embedding_bwd_rank", st);
-        embed_rank_kernel<ID><<<(int)up(M, kRankTokens), kThreads, 0, st>>>(ids, (int)M,
-                                                                            (uint32_t)V, *keys,
-                                                                            *order);
+        embed_rank_kernel<ID><<<z.first + z.blocks, kThreads, 0, st>>>(ids, (int)M, (uint32_t)V,
+                                                                       *keys, *order, z);
         return;
     }
+    const bool few = p.tiles <= kFewTiles;
+    const Counts counts = {at(p.counts), p.tiles, few ? 1 : (size_t)p.tiles, few ? kDigits : (size_t)1};
     for (int pass = 0; pass < p.passes; ++pass) {
         uint32_t *to_keys = at(p.keys[pass & 1]), *to_order = at(p.order[pass & 1]);
         const auto run = [&](auto src) {
             KernelTimer timer("embedding_bwd_sort", st);
-            embed_count_kernel<<<(int)p.tiles, kThreads, 0, st>>>(src, M, 8 * pass, p.tiles,
-                                                                  at(p.counts));
-            embed_scan_kernel<<<kDigits, kThreads, 0, st>>>(at(p.counts), p.tiles, at(p.totals));
-            embed_scatter_kernel<<<(int)p.tiles, kThreads, 0, st>>>(
-                src, M, 8 * pass, p.tiles, at(p.counts), at(p.totals), to_keys, to_order);
+            Zero z = zero(2 * pass, p.tiles);
+            embed_count_kernel<<<z.first + z.blocks, kThreads, 0, st>>>(src, M, 8 * pass, counts,
+                                                                        z);
+            if (!few) embed_scan_kernel<<<kDigits, kThreads, 0, st>>>(counts, at(p.totals));
+            z = zero(2 * pass + 1, p.tiles);
+            embed_scatter_kernel<<<z.first + z.blocks, kThreads, 0, st>>>(
+                src, M, 8 * pass, counts, few ? nullptr : at(p.totals), to_keys, to_order, z);
         };
         if (pass == 0) run(FirstKeys<ID>{ids, (uint32_t)V});
         else run(NextKeys{*keys, *order});
@@ -834,17 +874,24 @@ void launch_sum(hipStream_t st, const void* dout, const uint32_t* keys, const ui
                 float scale) {
     using E = typename TR::elem;
     constexpr int N = Vec<TR>::N;
-    const int64_t slices = up(up(C, N), LPR);
-    const int64_t sum_blocks = up(p.chunks * slices, kThreads / LPR);
-    const int64_t grid = sum_blocks + up(V + 1, kThreads);
     const auto kernel = C % N == 0 ? embed_sum_kernel<TR, LPR, true>
                                    : embed_sum_kernel<TR, LPR, false>;
-    KernelTimer timer("embedding_bwd_sum", st);
-    kernel<<<(uint32_t)grid, kThreads, 0, st>>>(
-        static_cast<const E*>(dout), keys, order, dtable, reinterpret_cast<float*>(ws + p.head),
-        reinterpret_cast<float*>(ws + p.tail), reinterpret_cast<uint32_t*>(ws + p.starts),
-        (uint32_t)M, (uint32_t)V, (int)C, (uint32_t)p.chunks, fast_div((uint32_t)slices),
-        (uint32_t)sum_blocks, scale);
+    constexpr int tokens = chunk_tokens<LPR>();
+    const int64_t chunks = up(M, tokens), slices = up(up(C, N), LPR);
+    float* head = reinterpret_cast<float*>(ws + p.head);
+    float* tail = reinterpret_cast<float*>(ws + p.tail);
+    {
+        KernelTimer timer("embedding_bwd_sum", st);
+        kernel<<<(uint32_t)(chunks * slices), kThreads, 0, st>>>(
+            static_cast<const E*>(dout), keys, order, dtable, head, tail, (uint32_t)M, (uint32_t)V,
+            (int)C, fast_div((uint32_t)slices), scale);
+    }
+    if (chunks == 1) return;
+    const int64_t join_slices = up(C, 256);
+    KernelTimer timer("embedding_bwd_join", st);
+    embed_join_kernel<<<(uint32_t)((chunks - 1) * join_slices), kThreads, 0, st>>>(
+        keys, head, tail, dtable, (uint32_t)V, (int)C, (uint32_t)chunks, tokens,
+        fast_div((uint32_t)join_slices), scale);
 }
 
 template <typename TR, typename ID, int VT, int WC, bool WHOLE>
@@ -888,31 +935,13 @@ void launch_bwd(hipStream_t st, const void* dout, const void* ids, float* dtable
         return;
     }
     uint32_t *keys = nullptr, *order = nullptr;
-    sort_tokens<ID>(st, static_cast<const ID*>(ids), ws, p, M, V, &keys, &order);
-    // Lanes a row: as many as it has vectors, up to the 16 that read 256 bytes of it.
-    const int64_t nvec = up(C, N);
-    const auto sum = nvec > 8   ? launch_sum<TR, 16>
-                     : nvec > 4 ? launch_sum<TR, 8>
-                     : nvec > 2 ? launch_sum<TR, 4>
-                                : launch_sum<TR, 2>;
+    sort_tokens<ID>(st, static_cast<const ID*>(ids), dtable, ws, p, M, V, C, &keys, &order);
+    const int lanes = lanes_a_row(up(C, N));
+    const auto sum = lanes == 16  ? launch_sum<TR, 16>
+                     : lanes == 8 ? launch_sum<TR, 8>
+                     : lanes == 4 ? launch_sum<TR, 4>
+                                  : launch_sum<TR, 2>;
     sum(st, dout, keys, order, dtable, ws, p, M, V, C, scale);
-    const float* head = reinterpret_cast<const float*>(ws + p.head);
-    const float* tail = reinterpret_cast<const float*>(ws + p.tail);
-    const uint32_t* starts = reinterpret_cast<const uint32_t*>(ws + p.starts);
-    const int64_t slices = up(C, 256);
-    {
-        KernelTimer timer("embedding_bwd_join", st);
-        const int64_t grid = std::min<int64_t>(up(V * slices, kThreads / 64), kMaxBlocks);
-        embed_join_kernel<<<(uint32_t)grid, kThreads, 0, st>>>(
-            head, tail, starts, dtable, (uint32_t)V, (int)C, fast_div((uint32_t)slices), scale);
-    }
-    const int64_t marks = (p.chunks - 1) / kLongRun;  // multiples of kLongRun past chunk 0
-    if (marks > 0) {
-        KernelTimer timer("embedding_bwd_join_long", st);
-        embed_join_long_kernel<<<dim3((uint32_t)marks, (uint32_t)slices), 64 * kLongWaves, 0,
-                                 st>>>(keys, head, tail, starts, dtable, (uint32_t)V, (int)C,
-                                       scale);
-    }
 }
 
 // fn<TR, ID> for the two types of a call.

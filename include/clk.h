@@ -335,8 +335,8 @@ clk_status clk_triangle_multiply(hipStream_t stream, clk_dtype dtype, const void
  * Token embedding (new; the residue types, MSA tokens and relative positions that the blocks'
  * representations begin from): out[i] = scale * table[ids[i]]. An id outside [0, V) is an absent
  * token: its row of out is zero. table and out of dtype CLK_F16, CLK_BF16 or CLK_F32, 16-byte
- * aligned; ids of ids_dtype CLK_S32 or CLK_S64. Any C up to 2^20; M and V below 2^30, M*C up to
- * 2^38, V*C up to 2^37.
+ * aligned; ids of ids_dtype CLK_S32 or CLK_S64. Any C up to 2^20; M up to 2^30, V below 2^30,
+ * M*C and V*C up to 2^37.
  */
 clk_status clk_embedding_fwd(hipStream_t stream, clk_dtype dtype, const void* table,
                              clk_dtype ids_dtype, const void* ids, void* out, int64_t M,

@@ -194,3 +194,49 @@ def test_autograd_and_streams(cuda):
     y = ops.EmbeddingFunction.apply(table, ids, 8.0)
     grad, = torch.autograd.grad(y.sum(), table)
     assert torch.equal(grad, ops.embedding_bwd(torch.ones_like(dout), ids, 40, 8.0).bfloat16())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,v,c", [
+    (2048, 145, 8), (2049, 500, 16), (8192, 1000, 40), (16384, 3000, 24), (20481, 145, 72),
+    (65536, 100000, 8), (65537, 200, 8), (70001, 255, 17), (70001, 256, 8), (140000, 70000, 12),
+    (70000, 20_000_000, 1)])
+@pytest.mark.parametrize("law", ["uniform", "long_tail", "one"])
+def test_gradient_by_sorted_tokens(cuda, dtype, m, v, c, law):
+    """Every way of sorting, at its first and last number of tokens, and of 1 to 4 digits of ids."""
+    g = torch.Generator().manual_seed(m + v)
+    dout = torch.randn(m, c, generator=g).to(dtype).to(cuda)
+    ids = make_ids(m, v, law, g, torch.int64 if m % 2 else torch.int32, 0.1).to(cuda)
+    got = ops.embedding_bwd(dout, ids, v, 0.5)
+    if v > 10 ** 6:  # compare the rows that are named; the others are zero
+        there = ids[(ids >= 0) & (ids < v)].unique().long()
+        named = torch.zeros(v, dtype=torch.bool, device=cuda)
+        named[there] = True
+        assert not got[~named].any()
+        index = torch.full((v + 1,), -1, device=cuda)
+        index[there] = torch.arange(len(there), device=cuda)
+        ids = torch.where((ids >= 0) & (ids < v), index[ids.clamp(0, v - 1)], -1)
+        got, v = got[there], len(there)
+    check_gradient(got, dout, ids, v, 0.5)
+
+
+@pytest.mark.parametrize("seed", range(4))
+@pytest.mark.parametrize("c", [4, 300])
+def test_gradient_of_runs_of_all_lengths(cuda, seed, c):
+    """Runs of equal tokens that end on, before and behind the multiples of any chunk of the sorted
+    order, up to thousands of tokens, after a shift of 0 to 40 tokens."""
+    rng = np.random.default_rng(seed)
+    lengths = [1, 2, 7, 8, 9, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 500, 511, 512, 513,
+               1007, 1008, 1009, 1023, 1024, 1025, 1040, 1041, 2047, 2048, 2049, 2064, 3100, 5000]
+    rng.shuffle(lengths)
+    lengths = [int(rng.integers(0, 41))] + lengths
+    ids = np.repeat(np.arange(len(lengths)) * 7 + 3, lengths)
+    v = 7 * len(lengths) + 150
+    order = rng.permutation(len(ids))
+    ids = torch.from_numpy(ids[order]).to(cuda)
+    dout = torch.randn(len(ids), c, generator=torch.Generator().manual_seed(seed)).to(cuda)
+    got = ops.embedding_bwd(dout, ids, v)
+    check_gradient(got, dout, ids, v, 1.0)
+    # The order of a row's sum is that of its tokens: another mix of the rows gives the same bits.
+    back = torch.argsort(ids, stable=True)
+    assert torch.equal(got, ops.embedding_bwd(dout[back].contiguous(), ids[back].contiguous(), v))
