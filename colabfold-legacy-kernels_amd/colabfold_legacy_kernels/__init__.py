@@ -10,8 +10,9 @@ Differences, all supersets of the reference contract:
     capabilities 70/75/80 resolve to no library, so ``available(75)`` is False on this build;
   * the three reference kernels keep their FFI target names (VoltaMma, VoltaLayerNorm,
     VoltaGdp), so a caller that registers ``symbol(kernel, cc)`` needs no change;
-  * three kernels the reference lacks are added: the attention backward, the LayerNorm backward
-    and LayerNorm fused with both gated-projection branches.
+  * kernels the reference lacks are added: the backward passes, LayerNorm fused with both
+    gated-projection branches, the gate, the pair bias, the triangle multiplication, the token
+    embedding and the residual join with its norms.
 """
 
 from pathlib import Path
@@ -50,6 +51,10 @@ _TABLE = {
     "ln_pair_bias": ((_ARCH, _LIB, "ClkLnPairBias"),),
     "gated_dual_proj_bwd": ((_ARCH, _LIB, "ClkGdpBwd"),),
     "triangle_multiply": ((_ARCH, _LIB, "ClkTriangleMultiply"),),
+    "embedding": ((_ARCH, _LIB, "ClkEmbedding"),),
+    "embedding_bwd": ((_ARCH, _LIB, "ClkEmbeddingBwd"),),
+    "residual_norm": ((_ARCH, _LIB, "ClkResidualNorm"),),
+    "residual_norm_bwd": ((_ARCH, _LIB, "ClkResidualNormBwd"),),
 }
 
 KERNELS = tuple(_TABLE)

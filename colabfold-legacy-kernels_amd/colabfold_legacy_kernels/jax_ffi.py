@@ -9,7 +9,7 @@ The reference leaves registration to its caller; the caller's code for the refer
 for each kernel k. This helper does the same for gfx950 with platform "ROCM", for the
 reference's targets (VoltaMma, VoltaWmma, VoltaLayerNorm, VoltaGdp, VoltaGdpWmma) and for the
 targets the reference lacks (the backward passes, fused LayerNorm + projections, the gate, the
-pair bias, the triangle multiplication). jax is imported only when register() runs.
+pair bias, the triangle multiplication, the embedding, the residual join). jax is imported only when register() runs.
 """
 
 import ctypes

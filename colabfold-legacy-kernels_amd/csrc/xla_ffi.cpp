@@ -34,6 +34,17 @@
 //                     six weights [C,C], six biases [C] -> out [N,N,C], workspace (u8,
 //                     clk_triangle_multiply_workspace_size bytes); attributes eps (f32), outgoing
 //                     (i64, 1 = 'ikc,jkc->ijc', 0 = 'kjc,kic->ijc')
+//   ClkEmbedding      table [V,C], ids (s32 or s64, any shape) -> out [ids..., C]; attribute scale
+//   ClkEmbeddingBwd   dout [ids..., C], ids -> dtable (f32 [V,C]), workspace (u8,
+//                     clk_embedding_bwd_workspace_size bytes); attribute scale
+//   ClkResidualNorm   x, o [..., C], then what the attributes say: gate [..., C] (gate = 1), the
+//                     norm after the block (post = 1: scale, 2: scale and offset), the residual
+//                     scale (res_scale = 1), the norm before the next block (pre = 1 or 2), vectors
+//                     f32 [C] -> r, and h with pre; attributes also rms (i64, 0 LayerNorm, 1 RMS
+//                     norm) and eps
+//   ClkResidualNormBwd  r, o, the same operands in the same order, dr, and dh with pre -> dx, do,
+//                     [dgate], the gradients of the vectors in their order (f32 [C]), workspace (u8,
+//                     clk_residual_norm_bwd_workspace_size bytes); the same attributes
 #include <hip/hip_runtime.h>
 
 #include <cstring>
@@ -550,6 +561,163 @@ clk_status triangle_multiply(const Frame& f) {
                                  outgoing != 0, eps);
 }
 
+bool whole_type(DataType t) { return t == kF16 || t == kBF16 || t == kF32; }
+
+// Whether `rows` is `ids` with one more axis, C.
+bool rows_of(const Buffer* rows, const Buffer* ids, int64_t C) {
+    if (!rows || rows->rank != ids->rank + 1 || rows->dims[ids->rank] != C) return false;
+    for (int64_t i = 0; i < ids->rank; ++i)
+        if (rows->dims[i] != ids->dims[i]) return false;
+    return true;
+}
+
+clk_status embedding(const Frame& f) {
+    const char* who = "ClkEmbedding";
+    const Buffer *table = f.arg(0), *ids = f.arg(1), *out = f.ret(0);
+    if (f.nargs() != 2 || f.nrets() != 1 || !table || !ids || !out)
+        return bad(who, "expects table, ids -> out");
+    if (table->rank != 2 || !whole_type(table->dtype))
+        return bad(who, "table must be [V,C] of f16, bf16 or f32");
+    if (ids->dtype != kS32 && ids->dtype != kS64) return bad(who, "ids must be s32 or s64");
+    const int64_t V = table->dims[0], C = table->dims[1];
+    if (!rows_of(out, ids, C) || out->dtype != table->dtype)
+        return bad(who, "out must be ids' shape and [C] of the table's dtype");
+    float scale;
+    if (!f.attr_f32("scale", &scale)) return bad(who, "missing f32 attribute 'scale'");
+    return clk_embedding_fwd(f.stream(), static_cast<clk_dtype>(table->dtype), table->data,
+                             static_cast<clk_dtype>(ids->dtype), ids->data, out->data, numel(ids),
+                             V, C, scale);
+}
+
+clk_status embedding_bwd(const Frame& f) {
+    const char* who = "ClkEmbeddingBwd";
+    const Buffer *dout = f.arg(0), *ids = f.arg(1), *dt = f.ret(0), *ws = f.ret(1);
+    if (f.nargs() != 2 || f.nrets() != 2 || !dout || !ids || !dt || !ws)
+        return bad(who, "expects dout, ids -> dtable, workspace");
+    if (dt->rank != 2 || dt->dtype != kF32) return bad(who, "dtable must be f32 [V,C]");
+    if (ids->dtype != kS32 && ids->dtype != kS64) return bad(who, "ids must be s32 or s64");
+    const int64_t V = dt->dims[0], C = dt->dims[1];
+    if (!rows_of(dout, ids, C) || !whole_type(dout->dtype))
+        return bad(who, "dout must be ids' shape and [C] of f16, bf16 or f32");
+    if (ws->dtype != kU8) return bad(who, "second result must be the u8 workspace");
+    float scale;
+    if (!f.attr_f32("scale", &scale)) return bad(who, "missing f32 attribute 'scale'");
+    return clk_embedding_bwd(f.stream(), static_cast<clk_dtype>(dout->dtype), dout->data,
+                             static_cast<clk_dtype>(ids->dtype), ids->data,
+                             static_cast<float*>(dt->data), ws->data, (size_t)numel(ws),
+                             numel(ids), V, C, scale);
+}
+
+// The operands of the residual join behind its first two, as the attributes list them.
+struct JoinOperands {
+    int64_t gate = 0, post = 0, res_scale = 0, pre = 0, rms = 0;
+    float eps = 0.f;
+    const void* gate_rows = nullptr;
+    const float *post_scale = nullptr, *post_offset = nullptr, *scale = nullptr,
+                *pre_scale = nullptr, *pre_offset = nullptr;
+    int64_t M = 0, C = 0, next = 2;  // the next operand
+    clk_dtype dtype = CLK_F32;
+};
+
+bool same_rows(const Buffer* b, const Buffer* first) {
+    if (!b || b->rank != first->rank || b->dtype != first->dtype) return false;
+    for (int64_t i = 0; i < b->rank; ++i)
+        if (b->dims[i] != first->dims[i]) return false;
+    return true;
+}
+
+clk_status decode_join(const char* who, const Frame& f, JoinOperands* j) {
+    const Buffer *x = f.arg(0), *o = f.arg(1);
+    if (!x || x->rank < 1 || !whole_type(x->dtype) || !same_rows(o, x))
+        return bad(who, "the first two operands must be [..., C] of f16, bf16 or f32, alike");
+    j->C = x->dims[x->rank - 1];
+    j->M = j->C ? numel(x) / j->C : 0;
+    j->dtype = static_cast<clk_dtype>(x->dtype);
+    if (!f.attr_i64("gate", &j->gate) || !f.attr_i64("post", &j->post) ||
+        !f.attr_i64("res_scale", &j->res_scale) || !f.attr_i64("pre", &j->pre) ||
+        !f.attr_i64("rms", &j->rms) || !f.attr_f32("eps", &j->eps))
+        return bad(who, "missing i64 attributes 'gate', 'post', 'res_scale', 'pre', 'rms' or f32 "
+                        "attribute 'eps'");
+    if (j->gate < 0 || j->gate > 1 || j->post < 0 || j->post > 2 || j->res_scale < 0 ||
+        j->res_scale > 1 || j->pre < 0 || j->pre > 2)
+        return bad(who, "gate and res_scale must be 0 or 1, post and pre 0, 1 or 2");
+    if (j->gate) {
+        const Buffer* g = f.arg(j->next++);
+        if (!same_rows(g, x)) return bad(who, "gate must match the first operand");
+        j->gate_rows = g->data;
+    }
+    const struct {
+        bool there;
+        const float** to;
+    } vectors[] = {{j->post > 0, &j->post_scale}, {j->post > 1, &j->post_offset},
+                   {j->res_scale > 0, &j->scale}, {j->pre > 0, &j->pre_scale},
+                   {j->pre > 1, &j->pre_offset}};
+    for (const auto& v : vectors) {
+        if (!v.there) continue;
+        const Buffer* b = f.arg(j->next++);
+        if (!dims_are(b, {j->C}) || b->dtype != kF32)
+            return bad(who, "norm scales and offsets and the residual scale must be f32 [C]");
+        *v.to = static_cast<const float*>(b->data);
+    }
+    return CLK_OK;
+}
+
+clk_norm norm_of(const JoinOperands& j) {
+    return j.rms == 0 ? CLK_NORM_LAYER : j.rms == 1 ? CLK_NORM_RMS : static_cast<clk_norm>(-1);
+}
+
+clk_status residual_norm(const Frame& f) {
+    const char* who = "ClkResidualNorm";
+    JoinOperands j;
+    const clk_status s = decode_join(who, f, &j);
+    if (s != CLK_OK) return s;
+    if (f.nargs() != j.next || f.nrets() != (j.pre ? 2 : 1))
+        return bad(who, "operands or results do not match the attributes");
+    const Buffer *r = f.ret(0), *h = j.pre ? f.ret(1) : nullptr;
+    if (!same_rows(r, f.arg(0)) || (j.pre && !same_rows(h, f.arg(0))))
+        return bad(who, "results must match the first operand");
+    return clk_residual_norm_fwd(f.stream(), j.dtype, norm_of(j), f.arg(0)->data, f.arg(1)->data,
+                                 j.gate_rows, j.post_scale, j.post_offset, j.scale, j.pre_scale,
+                                 j.pre_offset, r->data, h ? h->data : nullptr, j.M, j.C, j.eps);
+}
+
+clk_status residual_norm_bwd(const Frame& f) {
+    const char* who = "ClkResidualNormBwd";
+    JoinOperands j;
+    const clk_status s = decode_join(who, f, &j);
+    if (s != CLK_OK) return s;
+    const int64_t sums = j.post + j.res_scale + j.pre;
+    if (f.nargs() != j.next + 1 + (j.pre ? 1 : 0) || f.nrets() != 2 + j.gate + sums + 1)
+        return bad(who, "operands or results do not match the attributes");
+    const Buffer *first = f.arg(0), *dr = f.arg(j.next),
+                 *dh = j.pre ? f.arg(j.next + 1) : nullptr;
+    if (!same_rows(dr, first) || (j.pre && !same_rows(dh, first)))
+        return bad(who, "dr and dh must match r");
+    void* rows[3] = {nullptr, nullptr, nullptr};
+    for (int64_t i = 0; i < 2 + j.gate; ++i) {
+        if (!same_rows(f.ret(i), first)) return bad(who, "dx, do and dgate must match r");
+        rows[i] = f.ret(i)->data;
+    }
+    // In the order of the operands: post scale and offset, residual scale, pre scale and offset.
+    float* to[5] = {};
+    const bool there[5] = {j.post > 0, j.post > 1, j.res_scale > 0, j.pre > 0, j.pre > 1};
+    int64_t at = 2 + j.gate;
+    for (int i = 0; i < 5; ++i) {
+        if (!there[i]) continue;
+        const Buffer* b = f.ret(at++);
+        if (!dims_are(b, {j.C}) || b->dtype != kF32)
+            return bad(who, "gradients of norms and of the residual scale must be f32 [C]");
+        to[i] = static_cast<float*>(b->data);
+    }
+    const Buffer* ws = f.ret(at);
+    if (!ws || ws->dtype != kU8) return bad(who, "the last result must be the u8 workspace");
+    return clk_residual_norm_bwd(f.stream(), j.dtype, norm_of(j), first->data, f.arg(1)->data,
+                                 j.gate_rows, j.post_scale, j.post_offset, j.scale, j.pre_scale,
+                                 dr->data, dh ? dh->data : nullptr, rows[0], rows[1], rows[2],
+                                 to[0], to[1], to[2], to[3], to[4], ws->data, (size_t)numel(ws),
+                                 j.M, j.C, j.eps);
+}
+
 }  // namespace
 
 #define CLK_FFI_EXPORT extern "C" __attribute__((visibility("default")))
@@ -604,4 +772,16 @@ CLK_FFI_EXPORT Error* ClkGdpBwd(CallFrame* frame) {
 }
 CLK_FFI_EXPORT Error* ClkTriangleMultiply(CallFrame* frame) {
     return run(frame, [](const Frame& f) { return triangle_multiply(f); });
+}
+CLK_FFI_EXPORT Error* ClkEmbedding(CallFrame* frame) {
+    return run(frame, [](const Frame& f) { return embedding(f); });
+}
+CLK_FFI_EXPORT Error* ClkEmbeddingBwd(CallFrame* frame) {
+    return run(frame, [](const Frame& f) { return embedding_bwd(f); });
+}
+CLK_FFI_EXPORT Error* ClkResidualNorm(CallFrame* frame) {
+    return run(frame, [](const Frame& f) { return residual_norm(f); });
+}
+CLK_FFI_EXPORT Error* ClkResidualNormBwd(CallFrame* frame) {
+    return run(frame, [](const Frame& f) { return residual_norm_bwd(f); });
 }
