@@ -88,7 +88,7 @@ __device__ __forceinline__ void load_half4(const void* p, uint32_t at, uint32_t 
     using E = typename TR::elem;
     const auto e = global<const E>(p);
     if (FULL) {
-        const u32x2 raw = *(Global<const u32x2_a2>)(e + at);
+        const u32x2 raw = __builtin_nontemporal_load((Global<const u32x2_a2>)(e + at));
         E h[4];
         __builtin_memcpy(h, &raw, 8);
 #pragma unroll
@@ -104,7 +104,7 @@ template <bool FULL>
 __device__ __forceinline__ void load_float4(const void* p, uint32_t at, uint32_t n, float (&x)[4]) {
     const auto e = global<const float>(p);
     if (FULL) {
-        const f32x4 v = *(Global<const f32x4_a4>)(e + at);
+        const f32x4 v = __builtin_nontemporal_load((Global<const f32x4_a4>)(e + at));
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[i] = v[i];
     } else {

@@ -54,7 +54,7 @@ __global__ __launch_bounds__(kThreads) void embed_kernel(
                     for (int i = 0; i < N; ++i) v[i] *= scale;
                     raw[u] = pack_vec<TR>(v);
                 }
-                store_vec<TR, WHOLE>(out + (size_t)(row0 + r[u]) * C, col[u], C, raw[u]);
+                store_vec<TR, WHOLE, true>(out + (size_t)(row0 + r[u]) * C, col[u], C, raw[u]);
             }
         }
     }

@@ -14,10 +14,12 @@ struct Vec {
     static constexpr int N = 16 / sizeof(typename TR::elem);
 };
 
-// The N elements from `col` on, zero past the row's end.
-template <typename TR, bool WHOLE>
+// The N elements from `col` on, zero past the row's end. NT: non-temporal where a vector is aligned
+// (rows that are read once).
+template <typename TR, bool WHOLE, bool NT = false>
 __device__ __forceinline__ u32x4 load_vec(const typename TR::elem* row, int col, int C) {
     constexpr int N = Vec<TR>::N;
+    if (WHOLE && NT) return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(row + col));
     if (WHOLE) return ld16(row + col);
     if (col + N <= C) return ld16_a2(row + col);
     typename TR::elem e[N];
@@ -46,12 +48,14 @@ __device__ __forceinline__ u32x4 pack_vec(const float (&v)[Vec<TR>::N]) {
     return raw;
 }
 
-// Stores of results that the kernel does not read again (non-temporal where a vector is aligned).
-template <typename TR, bool WHOLE>
+// Stores, non-temporal with NT where a vector is aligned.
+template <typename TR, bool WHOLE, bool NT>
 __device__ __forceinline__ void store_vec(typename TR::elem* row, int col, int C, u32x4 raw) {
     constexpr int N = Vec<TR>::N;
-    if (WHOLE) {
+    if (WHOLE && NT) {
         __builtin_nontemporal_store(raw, reinterpret_cast<u32x4*>(row + col));
+    } else if (WHOLE) {
+        st16(row + col, raw);
     } else if (col + N <= C) {
         *reinterpret_cast<u32x4_a2*>(row + col) = raw;
     } else {
