@@ -621,7 +621,7 @@ _NORMS = {"layer": _native.NORM_LAYER, "rms": _native.NORM_RMS}
 _ROW_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
 
 
-def _residual_args(rows, gate, post, res_scale, pre, kind, what):
+def _residual_args(rows, post, res_scale, pre, kind, what):
     """(device, dtype code, norm code, M, C, post scale, post offset, pre scale, pre offset) of
     residual_norm's operands; each tensor is looked at once."""
     first = rows[0][1]
@@ -633,27 +633,25 @@ def _residual_args(rows, gate, post, res_scale, pre, kind, what):
         _fail(what, "dtype %s not supported" % dtype)
     if kind not in _NORMS:
         _fail(what, "kind must be 'layer' or 'rms', got %r" % (kind,))
-    for name, t in rows + (("gate", gate),):
-        if t is None:
-            continue
-        if not isinstance(t, torch.Tensor) or t.get_device() != index:
-            _fail(what, "%s must be a tensor on the device of %s" % (name, rows[0][0]))
-        if t.shape != shape or t.dtype != dtype:
-            _fail(what, "%s must match %s" % (name, rows[0][0]))
-        if not t.is_contiguous():
-            _fail(what, "%s must be contiguous" % name)
     post_scale, post_offset = post if post is not None else (None, None)
     pre_scale, pre_offset = pre if pre is not None else (None, None)
     if (post is not None and post_scale is None) or (pre is not None and pre_scale is None):
         _fail(what, "a norm needs a scale")
-    for name, t in (("post", post_scale), ("post", post_offset), ("res_scale", res_scale),
-                    ("pre", pre_scale), ("pre", pre_offset)):
-        if t is None:
-            continue
-        if not isinstance(t, torch.Tensor) or t.get_device() != index:
-            _fail(what, "%s must be on the device of %s" % (name, rows[0][0]))
-        if t.dtype != torch.float32 or t.dim() != 1 or t.numel() != c or not t.is_contiguous():
-            _fail(what, "%s must be float32 [C], contiguous" % name)
+    if rows[1][1] is None:
+        _fail(what, "%s must be given" % rows[1][0])
+    vector, f32 = (c,), torch.float32
+    try:
+        for name, t in rows:
+            if t is not None and (t.shape != shape or t.dtype != dtype or t.get_device() != index or
+                                  not t.is_contiguous()):
+                _fail(what, "%s must match %s, contiguous and on its device" % (name, rows[0][0]))
+        for t in (post_scale, post_offset, res_scale, pre_scale, pre_offset):
+            if t is not None and (t.shape != vector or t.dtype != f32 or
+                                  t.get_device() != index or not t.is_contiguous()):
+                _fail(what, "norm scales and offsets and res_scale must be float32 [C], "
+                            "contiguous and on the device of %s" % rows[0][0])
+    except AttributeError:
+        _fail(what, "operands must be tensors")
     return (index, _DTYPES[dtype], _NORMS[kind], first.numel() // c if c else 0, c, post_scale,
             post_offset, pre_scale, pre_offset)
 
@@ -665,7 +663,7 @@ def residual_norm(x, o, gate=None, post=None, res_scale=None, pre=None, kind="la
     or, with kind "rms", of an RMS norm, the offset None where there is none; res_scale float32 [C].
     gate, post, res_scale and pre may each be None: no gate, no norm, 1, no norm."""
     (index, code, norm, m, c, post_scale, post_offset, pre_scale, pre_offset) = _residual_args(
-        (("x", x), ("o", o)), gate, post, res_scale, pre, kind, "residual_norm")
+        (("x", x), ("o", o), ("gate", gate)), post, res_scale, pre, kind, "residual_norm")
     r = torch.empty_like(x)
     h = torch.empty_like(x) if pre_scale is not None else None
     _launch(index, _native.lib().clk_residual_norm_fwd, code, norm, x.data_ptr(), o.data_ptr(),
@@ -681,20 +679,21 @@ def residual_norm_bwd(r, o, gate, post, res_scale, pre, dr, dh, kind="layer", ep
     float32 [C], None for what was not given."""
     what = "residual_norm_bwd"
     (index, code, norm, m, c, post_scale, post_offset, pre_scale, pre_offset) = _residual_args(
-        (("r", r), ("o", o), ("dr", dr), ("dh", dh)), gate, post, res_scale, pre, kind, what)
+        (("r", r), ("o", o), ("gate", gate), ("dr", dr), ("dh", dh)), post, res_scale, pre, kind,
+        what)
     if (dh is not None) != (pre_scale is not None):
         _fail(what, "dh is given with pre, and only with it")
     if dr is None and dh is None:
         _fail(what, "dr or dh must be given")
     lib = _native.lib()
     wsb = lib.clk_residual_norm_bwd_workspace_size(m, c)
-    ws = r.new_empty(max(wsb, 1), dtype=torch.uint8)
-    dx, do = torch.empty_like(r), torch.empty_like(r)
-    dgate = torch.empty_like(r) if gate is not None else None
-    vectors = (post_scale, post_offset, res_scale, pre_scale, pre_offset)
+    ws = _workspace(r, wsb)
+    empty_like = torch.empty_like
+    dx, do, dgate = empty_like(r), empty_like(r), empty_like(r) if gate is not None else None
     sums = iter(r.new_empty((5, c), dtype=torch.float32).unbind(0))
     dpost_scale, dpost_offset, dres, dpre_scale, dpre_offset = [
-        None if t is None else next(sums) for t in vectors]
+        None if t is None else next(sums)
+        for t in (post_scale, post_offset, res_scale, pre_scale, pre_offset)]
     _launch(index, lib.clk_residual_norm_bwd, code, norm, r.data_ptr(), o.data_ptr(), _ptr(gate),
             _ptr(post_scale), _ptr(post_offset), _ptr(res_scale), _ptr(pre_scale), _ptr(dr),
             _ptr(dh), dx.data_ptr(), do.data_ptr(), _ptr(dgate), _ptr(dpost_scale),

@@ -328,10 +328,12 @@ __global__ __launch_bounds__(kThreads) void embed_sum_kernel(
     const bool cols = col < C;
     const uint32_t beg = chunk * chunk_tokens<LPR>() + g * kRun;
     const uint32_t end = beg >= M ? beg : M - beg < kRun ? M : beg + kRun;
-    uint32_t cur = beg < M ? keys[beg] : V;
+    // The keys around the group, loaded at once.
+    const uint32_t before = keys[beg > 0 && beg < M ? beg - 1 : 0], after = keys[min(end, M - 1)];
+    uint32_t cur = beg < M ? keys[min(beg, M - 1)] : V;
     if (s == 0) first_key[g] = cur;
     // A head run began before the group; the last run goes on behind it.
-    const bool has_head = beg > 0 && beg < M && cur < V && keys[beg - 1] == cur;
+    const bool has_head = beg > 0 && cur < V && before == cur;
     bool began = !has_head, has_tail = false;
     float acc[N];
 #pragma unroll
@@ -378,7 +380,7 @@ __global__ __launch_bounds__(kThreads) void embed_sum_kernel(
     if (cur < V) {
         if (!began) {
             keep(heads[g]);
-        } else if (end < M && keys[end] == cur) {
+        } else if (end < M && after == cur) {
             has_tail = true;
         } else {
             finish(cur);
@@ -398,10 +400,10 @@ __global__ __launch_bounds__(kThreads) void embed_sum_kernel(
         for (; j < G && first_key[j] == key; ++j)
 #pragma unroll
             for (int i = 0; i < N; ++i) sum[i] += heads[j][s * N + i];
-        const uint32_t after = (chunk + 1) * chunk_tokens<LPR>();
+        const uint32_t next = (chunk + 1) * chunk_tokens<LPR>();
         float* to = head + (size_t)chunk * C;
         if (own == 1) {
-            const bool goes_on = j == G && after < M && keys[after] == key;
+            const bool goes_on = j == G && next < M && keys[next] == key;
             to = goes_on ? tail + (size_t)chunk * C : dtable + (size_t)key * C;
 #pragma unroll
             for (int i = 0; i < N; ++i) sum[i] *= goes_on ? 1.f : scale;
@@ -474,25 +476,36 @@ __global__ __launch_bounds__(kThreads) void embed_join_kernel(
 // adds its tokens up one by one instead.
 // ---------------------------------------------------------------------------------------------
 constexpr int kStep = 32, kHotWaves = 8, kHotCols = 64;
-constexpr int kHotRows = 144;  // most rows of a table that takes this path
+constexpr int kHotRows = 144;  // rows of a block; a table of more takes a block for each so many
+// Tables of up to kHotRows rows take this path, and larger ones where reading dout once for every
+// kHotRows rows costs less than the sort's launches: 4332 tokens of 496 rows of 256 columns @@ us
+// instead of 29.
+constexpr int64_t kHotSlices = 8, kHotWork = 1 << 23;
+inline bool hot_table(int64_t M, int64_t V, int64_t C) {
+    const int64_t slices = up(V, kHotRows);
+    return slices <= 1 ||
+           (slices <= kHotSlices && M * up(C, kHotCols) * kHotCols <= kHotWork / slices);
+}
 
+// A token's row counted from v0, -1 if it is not among the kHotRows rows from there on.
 template <typename ID>
-__device__ __forceinline__ int hot_id(ID id) {
-    return id >= 0 && id < (ID)kHotRows ? (int)id : -1;
+__device__ __forceinline__ int hot_id(ID id, int v0) {
+    return id >= (ID)v0 && id < (ID)(v0 + kHotRows) ? (int)(id - (ID)v0) : -1;
 }
 
 // Tokens t .. t + 7 of a lane.
 template <typename ID>
-__device__ __forceinline__ void load_ids8(const ID* ids, int64_t t, int64_t end, int (&id)[8]) {
+__device__ __forceinline__ void load_ids8(const ID* ids, int64_t t, int64_t end, int v0,
+                                          int (&id)[8]) {
     typedef ID ID4 __attribute__((ext_vector_type(4), aligned(sizeof(ID))));
     if (t + 8 <= end) {
         const ID4 a = *reinterpret_cast<const ID4*>(ids + t);
         const ID4 b = *reinterpret_cast<const ID4*>(ids + t + 4);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) id[j] = hot_id(a[j]), id[4 + j] = hot_id(b[j]);
+        for (int j = 0; j < 4; ++j) id[j] = hot_id(a[j], v0), id[4 + j] = hot_id(b[j], v0);
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) id[j] = t + j < end ? hot_id(ids[t + j]) : -1;
+        for (int j = 0; j < 8; ++j) id[j] = t + j < end ? hot_id(ids[t + j], v0) : -1;
     }
 }
 
@@ -578,6 +591,7 @@ __global__ __launch_bounds__(64 * kHotWaves) void embed_hot_kernel(
     const int64_t beg = (int64_t)blockIdx.x * tokens;
     const int64_t end = M - beg < tokens ? M : beg + tokens;
     const int64_t first = beg + (wave / WC) * kStep;
+    const int v0 = (int)blockIdx.z * kHotRows;
 
     f32x4 acc[VT][4];
 #pragma unroll
@@ -589,7 +603,7 @@ __global__ __launch_bounds__(64 * kHotWaves) void embed_hot_kernel(
     // past the last column load the first ones; their sums are not stored.
     const int lcol = col < C ? col : 0;
     const auto load = [&](int64_t t0, int(&id)[8], Four<TR>(&x)[8]) {
-        load_ids8(ids, t0 + 8 * g, end, id);
+        load_ids8(ids, t0 + 8 * g, end, v0, id);
         const typename TR::elem* base = dout + (size_t)t0 * C;
         const uint32_t off = (uint32_t)(8 * g * C);
         if (t0 + kStep <= end) {
@@ -645,7 +659,7 @@ __global__ __launch_bounds__(64 * kHotWaves) void embed_hot_kernel(
             for (int ct = 0; ct < 4; ++ct) acc[v][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
         for (int64_t t0 = first; t0 < end; t0 += WT * kStep)
             for (int64_t t = t0; t < end && t < t0 + kStep; ++t) {
-                const int id = hot_id(ids[t]);
+                const int id = hot_id(ids[t], v0);
                 if (id < 0 || col >= C || ((id >> 2) & 3) != g) continue;
                 const Four<TR> x = load_four<TR, WHOLE>(dout + (size_t)t * C, col, C);
 #pragma unroll
@@ -677,10 +691,10 @@ __global__ __launch_bounds__(64 * kHotWaves) void embed_hot_kernel(
 #pragma unroll
             for (int w = 1; w < WT; ++w)
                 sum += *reinterpret_cast<const f32x4*>(&red[w * WC + wc][row][c4]);
-            if (16 * v + row < V) {
+            if (v0 + 16 * v + row < V) {
                 const float s4[4] = {sum[0] * scale, sum[1] * scale, sum[2] * scale,
                                      sum[3] * scale};
-                store_floats<4>(to + (size_t)(16 * v + row) * C, cbase + 4 * q, C, s4);
+                store_floats<4>(to + (size_t)(v0 + 16 * v + row) * C, cbase + 4 * q, C, s4);
             }
         }
     }
@@ -754,12 +768,12 @@ struct BwdPlan {
 };
 BwdPlan bwd_plan(int64_t M, int64_t V, int64_t C) {
     BwdPlan p = {};
-    if (V <= kHotRows) {
-        // As many blocks as CUs, with at least four steps of tokens each.
+    if (hot_table(M, V, C)) {
+        // As many blocks as CUs, with at least two steps of tokens a wave.
         p.hot = true;
-        const int64_t cols = up(C, C > kHotCols ? 2 * kHotCols : kHotCols);
-        const int64_t want = std::max<int64_t>(1, 256 / cols);
-        const int64_t least = 4 * kStep * (C > kHotCols ? kHotWaves / 2 : kHotWaves);
+        const int64_t others = up(C, C > kHotCols ? 2 * kHotCols : kHotCols) * up(V, kHotRows);
+        const int64_t want = std::max<int64_t>(1, 256 / others);
+        const int64_t least = 2 * kStep * (C > kHotCols ? kHotWaves / 2 : kHotWaves);
         p.tokens = up(std::max(up(M, want), std::min(M, least)), kStep) * kStep;
         p.parts = (int)up(M, p.tokens);
         p.stride = (size_t)up(V * C, 4) * 4;
@@ -902,7 +916,8 @@ void launch_hot(hipStream_t st, const void* dout, const void* ids, float* dtable
     {
         KernelTimer timer("embedding_bwd_hot", st);
         embed_hot_kernel<TR, ID, VT, WC, WHOLE>
-            <<<dim3(p.parts, (uint32_t)up(C, kHotCols * WC)), 64 * kHotWaves, 0, st>>>(
+            <<<dim3(p.parts, (uint32_t)up(C, kHotCols * WC), (uint32_t)up(V, kHotRows)),
+               64 * kHotWaves, 0, st>>>(
                 static_cast<const E*>(dout), static_cast<const ID*>(ids),
                 p.parts > 1 ? parts : dtable, p.stride, M, (int)V, (int)C, p.tokens,
                 p.parts > 1 ? 1.f : scale);

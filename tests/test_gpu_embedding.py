@@ -235,8 +235,67 @@ def test_gradient_of_runs_of_all_lengths(cuda, seed, c):
     order = rng.permutation(len(ids))
     ids = torch.from_numpy(ids[order]).to(cuda)
     dout = torch.randn(len(ids), c, generator=torch.Generator().manual_seed(seed)).to(cuda)
+    check_gradient(ops.embedding_bwd(dout, ids, v), dout, ids, v, 1.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,v,c", [
+    (1, 5000, 16), (31, 5000, 9), (2048, 1153, 40), (4096, 5000, 8), (4097, 5000, 24),
+    (8192, 70000, 136), (32768, 5000, 20), (32769, 1153, 8), (40000, 70000, 72)])
+@pytest.mark.parametrize("law", ["long_tail", "one", "runs"])
+def test_gradient_of_larger_tables(cuda, dtype, m, v, c, law):
+    """Tables that are always sorted: by counting (up to 4096 tokens), by digits with few tiles of
+    tokens and with more."""
+    g = torch.Generator().manual_seed(m + v)
+    dout = torch.randn(m, c, generator=g).to(dtype).to(cuda)
+    ids = make_ids(m, v, law, g, torch.int64 if m % 2 else torch.int32, 0.1).to(cuda)
+    got = ops.embedding_bwd(dout, ids, v, 0.5)
+    check_gradient(got, dout, ids, v, 0.5)
+    assert torch.equal(got, ops.embedding_bwd(dout, ids, v, 0.5))
+
+
+@pytest.mark.parametrize("seed", range(6))
+@pytest.mark.parametrize("c", [2, 8, 20, 300])
+def test_gradient_of_sorted_runs_of_all_lengths(cuda, seed, c):
+    rng = np.random.default_rng(100 + seed)
+    lengths = [1, 2, 7, 8, 9, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 239, 240, 241, 255,
+               256, 257, 272, 500, 511, 512, 513, 1007, 1008, 1009, 1023, 1024, 1025, 1040, 1041,
+               2047, 2048, 2049, 2064, 4095, 4096, 4097, 5000]
+    rng.shuffle(lengths)
+    lengths = [int(rng.integers(0, 41))] + lengths[:6 if seed == 0 else 12 if seed == 1 else None]
+    ids = np.repeat(np.arange(len(lengths)) * 70 + 3, lengths)
+    v = 70 * len(lengths) + 1200
+    ids = torch.from_numpy(ids[rng.permutation(len(ids))]).to(cuda)
+    dout = torch.randn(len(ids), c, generator=torch.Generator().manual_seed(seed)).to(cuda)
     got = ops.embedding_bwd(dout, ids, v)
     check_gradient(got, dout, ids, v, 1.0)
-    # The order of a row's sum is that of its tokens: another mix of the rows gives the same bits.
+    # Where tokens are sorted, a row's sum has the order of its tokens: another mix of the rows
+    # gives the same bits.
     back = torch.argsort(ids, stable=True)
     assert torch.equal(got, ops.embedding_bwd(dout[back].contiguous(), ids[back].contiguous(), v))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("v", [143, 144, 145, 287, 288, 289, 1152])
+def test_gradient_at_the_borders_of_row_blocks(cuda, dtype, v):
+    """Small calls on tables of up to eight blocks of 144 rows; NaN and infinite gradients stay in
+    their rows, those of absent tokens reach nothing."""
+    g = torch.Generator().manual_seed(v)
+    m, c = 1500, 68
+    dout = torch.randn(m, c, generator=g).to(dtype).to(cuda)
+    ids = make_ids(m, v, "uniform", g, torch.int64, 0.2).to(cuda)
+    ids[:v] = torch.arange(min(v, m), device=cuda)
+    clean = ops.embedding_bwd(dout, ids, v, 0.5)
+    check_gradient(clean, dout, ids, v, 0.5)
+    dout[0], dout[142, 5] = float("nan"), float("inf")
+    dout[(ids < 0) | (ids >= v)] = float("nan")
+    got = ops.embedding_bwd(dout, ids, v, 0.5)
+    hit = torch.zeros(v, dtype=torch.bool, device=cuda)
+    hit[0] = hit[142] = True
+    size = ref.embedding_bwd(np.abs(np64(dout)), ids.cpu().numpy(), v, 0.5)
+    count = np.bincount(ids.cpu().numpy()[((ids >= 0) & (ids < v)).cpu().numpy()], minlength=v)
+    ok = (~hit).cpu().numpy()
+    err = np.abs(np64(got) - np64(clean))[ok]  # both in some order of the same float32 sums
+    assert (err <= 2 * (count[ok][:, None] + 3) * U32 * size[ok] + 1e-37).all()
+    assert got[0].isnan().all() and got[142, 5] == float("inf")
+    assert torch.isfinite(got[142, torch.arange(c, device=cuda) != 5]).all()
