@@ -478,8 +478,8 @@ __global__ __launch_bounds__(kThreads) void embed_join_kernel(
 constexpr int kStep = 32, kHotWaves = 8, kHotCols = 64;
 constexpr int kHotRows = 144;  // rows of a block; a table of more takes a block for each so many
 // Tables of up to kHotRows rows take this path, and larger ones where reading dout once for every
-// kHotRows rows costs less than the sort's launches: 4332 tokens of 496 rows of 256 columns @@ us
-// instead of 29.
+// kHotRows rows costs less than the sort's launches: 4332 tokens of 496 rows of 256 columns 20.5 us
+// instead of 29.2.
 constexpr int64_t kHotSlices = 8, kHotWork = 1 << 23;
 inline bool hot_table(int64_t M, int64_t V, int64_t C) {
     const int64_t slices = up(V, kHotRows);
@@ -766,14 +766,18 @@ struct BwdPlan {
     int64_t tiles, chunks;
     size_t keys[2], order[2], counts, totals, head, tail, bytes;
 };
-BwdPlan bwd_plan(int64_t M, int64_t V, int64_t C) {
+// `half`: dout has a 16-bit type (its calls need no more workspace than float32 ones).
+BwdPlan bwd_plan(int64_t M, int64_t V, int64_t C, bool half) {
     BwdPlan p = {};
     if (hot_table(M, V, C)) {
-        // As many blocks as CUs, with at least two steps of tokens a wave.
+        // As many blocks as CUs, with at least two steps of tokens a wave; up to eight where one
+        // block can then take all tokens and the partials' kernel is saved (the float32 products
+        // of eight steps would take longer than it).
         p.hot = true;
         const int64_t others = up(C, C > kHotCols ? 2 * kHotCols : kHotCols) * up(V, kHotRows);
         const int64_t want = std::max<int64_t>(1, 256 / others);
-        const int64_t least = 2 * kStep * (C > kHotCols ? kHotWaves / 2 : kHotWaves);
+        const int64_t round = kStep * (C > kHotCols ? kHotWaves / 2 : kHotWaves);
+        const int64_t least = half && M <= 8 * round ? M : 2 * round;
         p.tokens = up(std::max(up(M, want), std::min(M, least)), kStep) * kStep;
         p.parts = (int)up(M, p.tokens);
         p.stride = (size_t)up(V * C, 4) * 4;
@@ -933,7 +937,7 @@ template <typename TR, typename ID>
 void launch_bwd(hipStream_t st, const void* dout, const void* ids, float* dtable, char* ws,
                 int64_t M, int64_t V, int64_t C, float scale) {
     constexpr int N = Vec<TR>::N;
-    const BwdPlan p = bwd_plan(M, V, C);
+    const BwdPlan p = bwd_plan(M, V, C, sizeof(typename TR::elem) == 2);
     if (p.hot) {
         const auto pick = [&](auto vt, auto wc) {
             constexpr int VT = decltype(vt)::value, WC = decltype(wc)::value;
@@ -994,7 +998,7 @@ extern "C" clk_status clk_embedding_fwd(hipStream_t stream, clk_dtype dtype, con
 extern "C" size_t clk_embedding_bwd_workspace_size(int64_t M, int64_t V, int64_t C) {
     if (M <= 0 || V <= 0 || C <= 0 || validate("embedding_bwd", CLK_F32, CLK_S32, M, V, C) != CLK_OK)
         return 0;
-    return bwd_plan(M, V, C).bytes;
+    return bwd_plan(M, V, C, false).bytes;
 }
 
 extern "C" clk_status clk_embedding_bwd(hipStream_t stream, clk_dtype dtype, const void* dout,

@@ -260,9 +260,13 @@ __global__ __launch_bounds__(kThreads) void join_fwd_long(
     }
 }
 
+struct SumsOut {
+    float* to[kSums];
+};
+
 // Backward. A block walks its contiguous rows, ROWS at a time; each lane sums its columns over the
 // rows it meets, the block joins its row slots in order, and join_colsum adds the blocks' partial
-// rows part[block][sum][C4] in a fixed order.
+// rows part[block][sum][C4] in a fixed order; a block that is alone writes the results itself.
 template <typename E>
 struct BwdRows {
     const E *r, *o, *gate, *dr, *dh;
@@ -271,7 +275,8 @@ struct BwdRows {
 
 template <typename TR, int T, int NV, Fill FILL>
 __global__ __launch_bounds__(block_threads<T>()) void join_bwd_kernel(
-    BwdRows<typename TR::elem> a, float* __restrict__ part, int C4, int rows_per_block, Params p) {
+    BwdRows<typename TR::elem> a, float* __restrict__ part, int C4, int rows_per_block, Params p,
+    SumsOut result) {
     using L = Lane<TR, T, NV, FILL>;
     constexpr int N = L::N, ROWS = block_threads<T>() / T;
     __shared__ float lds[4 * (T > 64 ? T / 64 : 1)];
@@ -446,13 +451,17 @@ __global__ __launch_bounds__(block_threads<T>()) void join_bwd_kernel(
     }
 
     // Join the block's row slots, one sum at a time, in the order of the slots.
-    float* out = part + (size_t)blockIdx.x * kSums * C4;
+    const bool alone = gridDim.x == 1;
+    const auto sums_to = [&](int k) {
+        return alone ? result.to[k] : part + ((size_t)blockIdx.x * kSums + k) * C4;
+    };
     if constexpr (ROWS == 1) {
 #pragma unroll
         for (int k = 0; k < kSums; ++k)
 #pragma unroll
             for (int v = 0; v < NV; ++v)
-                if (lane.col(v) < p.C) store_floats<N>(out + (size_t)k * C4, lane.col(v), C4, acc[k][v]);
+                if (lane.has(v) && sums_to(k))
+                    store_floats<N>(sums_to(k), lane.col(v), alone ? p.C : C4, acc[k][v]);
     } else {
         __shared__ __attribute__((aligned(16))) float red[ROWS][PW];
 #pragma unroll
@@ -466,7 +475,7 @@ __global__ __launch_bounds__(block_threads<T>()) void join_bwd_kernel(
             for (int c = threadIdx.x; c < p.C; c += kThreads) {
                 float s = red[0][c];
                 for (int j = 1; j < ROWS; ++j) s += red[j][c];
-                out[(size_t)k * C4 + c] = s;
+                if (sums_to(k)) sums_to(k)[c] = s;
             }
         }
     }
@@ -561,9 +570,6 @@ __global__ __launch_bounds__(kThreads) void join_bwd_long(BwdRows<typename TR::e
     }
 }
 
-struct SumsOut {
-    float* to[kSums];
-};
 // out.to[k][c] = sum over the blocks' partial rows, in a fixed order: thread i adds rows i, i+256,
 // ..., a wave joins its lanes by a fixed butterfly and the four waves are added in order. Four
 // columns a block.
@@ -620,6 +626,8 @@ Team team_of(int64_t nvec, int want) {
 int64_t bwd_blocks(int64_t C) { return C <= 4096 ? 768 : 256; }
 int64_t bwd_rows_per_block(int64_t M, int64_t C, int t) {
     const int64_t slots = t > 64 ? 1 : kThreads / t;
+    // Up to four rounds of rows go to one block, which then needs no second launch.
+    if (M <= 4 * slots) return 4 * slots;
     return slots * up(up(M, slots), bwd_blocks(C));
 }
 
@@ -687,8 +695,9 @@ void launch_bwd(hipStream_t st, const void* r, const void* o, const void* gate, 
                 const int64_t rows = bwd_rows_per_block(p.M, p.C, T);
                 nblocks = (int)up(p.M, rows);
                 join_bwd_kernel<TR, T, decltype(nv)::value, decltype(w)::value>
-                    <<<nblocks, block_threads<T>(), 0, st>>>(a, part, C4, (int)rows, p);
+                    <<<nblocks, block_threads<T>(), 0, st>>>(a, part, C4, (int)rows, p, out);
             });
+        if (done && nblocks == 1) return;
         if (!done) {
             nblocks = (int)std::min<int64_t>(p.M, bwd_blocks(p.C));
             join_bwd_long<TR><<<nblocks, kThreads, 0, st>>>(a, part, C4, p);
