@@ -517,12 +517,18 @@ struct Four {
 template <typename TR, bool WHOLE>
 __device__ __forceinline__ Four<TR> load_four(const typename TR::elem* row, int col, int C) {
     using E = typename TR::elem;
+    constexpr int R = sizeof(E);  // 4-byte words
     typedef unsigned int raw_t
-        __attribute__((ext_vector_type(sizeof(E)), aligned(WHOLE ? 4 * sizeof(E) : sizeof(E))));
+        __attribute__((ext_vector_type(R), aligned(WHOLE ? 4 * sizeof(E) : sizeof(E))));
     Four<TR> f;
-    if (WHOLE || col + 4 <= C) {
-        const raw_t raw = *reinterpret_cast<const raw_t*>(row + col);
-        __builtin_memcpy(&f, &raw, sizeof(f));
+    if (WHOLE || C >= 4) {
+        // A partial vector as load_vec takes it.
+        const int at = WHOLE || col < C - 4 ? col : C - 4, s = col - at;
+        const raw_t raw = *reinterpret_cast<const raw_t*>(row + at);
+        u32x4 r = {raw[0], raw[1], 0u, 0u};
+        if (R == 4) r = u32x4{raw[0], raw[1], raw[R - 2], raw[R - 1]};
+        if (!WHOLE) r = R == 4 ? move_down4(r, s) : move_down2(r, s);
+        __builtin_memcpy(&f, &r, sizeof(f));
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) f.e[i] = col + i < C ? row[col + i] : TR::from_f(0.f);

@@ -83,12 +83,30 @@ struct Lane {
         return FILL == kExact || (WHOLE ? col(v) < C : col(v) + i < C);
     }
     __device__ __forceinline__ bool has(int v) const { return FILL == kExact || col(v) < C; }
-    __device__ __forceinline__ void load(const E* p, int64_t row, bool there,
-                                         u32x4 (&raw)[NV]) const {
+    // The loads of a row take no branch (a branch would wait for the loads in it before the next:
+    // 21.8 against 15.6 us in the backward of [2053, 449] float32). Vectors that do not exist are
+    // loaded from elsewhere in the row, and unpack makes them zeros. `row` has to exist.
+    __device__ __forceinline__ int from(int v) const {
+        return FILL == kPartial ? min(col(v), max(C - N, 0)) : has(v) ? col(v) : 0;
+    }
+    __device__ __forceinline__ void load(const E* p, int64_t row, u32x4 (&raw)[NV]) const {
+        if (FILL == kPartial && C < N) {  // the same for all rows
 #pragma unroll
-        for (int v = 0; v < NV; ++v)
-            raw[v] = there && has(v) ? load_vec<TR, WHOLE, true>(p + (size_t)row * C, col(v), C)
-                                     : u32x4{0u, 0u, 0u, 0u};
+            for (int v = 0; v < NV; ++v)
+                raw[v] = has(v) ? load_vec<TR, false>(p + (size_t)row * C, col(v), C) : u32x4{};
+            return;
+        }
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const E* e = p + (size_t)row * C + from(v);
+            raw[v] = WHOLE ? __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(e))
+                           : ld16_a2(e);
+        }
+    }
+    __device__ __forceinline__ void unpack(u32x4 raw, int v, bool there, float (&x)[N]) const {
+        if (FILL == kPartial && C >= N) raw = move_to<TR>(raw, min(from(v), col(v)), col(v));
+        if (!there || !has(v)) raw = u32x4{0u, 0u, 0u, 0u};
+        unpack_vec<TR>(raw, x);
     }
     // The forward's stores are non-temporal, the backward's are not: its three results then stay
     // in the caches beside the loads that pass them by.
@@ -160,12 +178,13 @@ __global__ __launch_bounds__(block_threads<T>()) void join_fwd_kernel(
         const int64_t row = row0 + slot;
         const bool there = row < p.M;
         u32x4 ro[NV], rx[NV], rg[NV];
-        lane.load(o, row, there, ro);
-        lane.load(x, row, there, rx);
-        if (gate) lane.load(gate, row, there, rg);
+        const int64_t in = there ? row : p.M - 1;
+        lane.load(o, in, ro);
+        lane.load(x, in, rx);
+        if (gate) lane.load(gate, in, rg);
         float t[NV][N], w[NV][N];
 #pragma unroll
-        for (int v = 0; v < NV; ++v) unpack_vec<TR>(ro[v], t[v]);
+        for (int v = 0; v < NV; ++v) lane.unpack(ro[v], v, there, t[v]);
         if (p.post_scale) {
             float mean, rstd, b[NV][N];
             row_stats<T>(lane, t, p, lds, turn, mean, rstd);
@@ -180,7 +199,7 @@ __global__ __launch_bounds__(block_threads<T>()) void join_fwd_kernel(
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
                 float g[N];
-                unpack_vec<TR>(rg[v], g);
+                lane.unpack(rg[v], v, there, g);
 #pragma unroll
                 for (int i = 0; i < N; ++i) t[v][i] *= sigmoid(g[i]);
             }
@@ -189,7 +208,7 @@ __global__ __launch_bounds__(block_threads<T>()) void join_fwd_kernel(
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             float xs[N];
-            unpack_vec<TR>(rx[v], xs);
+            lane.unpack(rx[v], v, there, xs);
 #pragma unroll
             for (int i = 0; i < N; ++i) xs[i] += w[v][i] * t[v][i];
             if (there) lane.template store<true>(r, row, v, xs);
@@ -288,10 +307,15 @@ __global__ __launch_bounds__(block_threads<T>()) void join_bwd_kernel(
     constexpr int PW = T * NV * N;  // columns that a team holds, at least C
     __shared__ __attribute__((aligned(16))) float prm[4][PW];
     for (int c = threadIdx.x; c < PW; c += block_threads<T>()) {
-        prm[0][c] = p.pre_scale && c < p.C ? p.pre_scale[c] : 0.f;
-        prm[1][c] = p.post_scale && c < p.C ? p.post_scale[c] : 0.f;
-        prm[2][c] = p.post_offset && c < p.C ? p.post_offset[c] : 0.f;
-        prm[3][c] = p.res_scale && c < p.C ? p.res_scale[c] : 1.f;
+        const int in = min(c, p.C - 1);
+        const float w0 = p.pre_scale ? p.pre_scale[in] : 0.f;
+        const float w1 = p.post_scale ? p.post_scale[in] : 0.f;
+        const float w2 = p.post_offset ? p.post_offset[in] : 0.f;
+        const float w3 = p.res_scale ? p.res_scale[in] : 1.f;
+        prm[0][c] = c < p.C ? w0 : 0.f;
+        prm[1][c] = c < p.C ? w1 : 0.f;
+        prm[2][c] = c < p.C ? w2 : 0.f;
+        prm[3][c] = w3;
     }
     __syncthreads();
     const auto from_lds = [&](int k, float (&w)[NV][N]) {
@@ -316,14 +340,14 @@ __global__ __launch_bounds__(block_threads<T>()) void join_bwd_kernel(
     // The next rows' loads are issued before the current rows' arithmetic.
     u32x4 nr[NV], no[NV], ng[NV], nd[NV], nh[NV];
     const auto fetch = [&](int64_t row) {
-        const bool there = row < end;
+        const int64_t in = row < end ? row : end - 1;
         if (p.pre_scale) {
-            lane.load(a.r, row, there, nr);
-            lane.load(a.dh, row, there, nh);
+            lane.load(a.r, in, nr);
+            lane.load(a.dh, in, nh);
         }
-        lane.load(a.o, row, there, no);
-        if (a.gate) lane.load(a.gate, row, there, ng);
-        if (a.dr) lane.load(a.dr, row, there, nd);
+        lane.load(a.o, in, no);
+        if (a.gate) lane.load(a.gate, in, ng);
+        if (a.dr) lane.load(a.dr, in, nd);
     };
     fetch(beg + slot);
     for (int64_t row0 = beg; row0 < end; row0 += ROWS) {
@@ -345,7 +369,7 @@ __global__ __launch_bounds__(block_threads<T>()) void join_bwd_kernel(
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             if (a.dr) {
-                unpack_vec<TR>(rd[v], d[v]);
+                lane.unpack(rd[v], v, there, d[v]);
             } else {
 #pragma unroll
                 for (int i = 0; i < N; ++i) d[v][i] = 0.f;
@@ -354,14 +378,14 @@ __global__ __launch_bounds__(block_threads<T>()) void join_bwd_kernel(
         if (p.pre_scale) {
             float y[NV][N], mean, rstd, s[2] = {0.f, 0.f};
 #pragma unroll
-            for (int v = 0; v < NV; ++v) unpack_vec<TR>(rr[v], y[v]);
+            for (int v = 0; v < NV; ++v) lane.unpack(rr[v], v, there, y[v]);
             row_stats<T>(lane, y, p, lds, turn, mean, rstd);
             if (!there) rstd = 0.f;  // eps = 0: a row of zeros has none
             from_lds(0, w);
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
                 float g[N];
-                unpack_vec<TR>(rh[v], g);
+                lane.unpack(rh[v], v, there, g);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     const float hat = (y[v][i] - mean) * rstd;
@@ -391,7 +415,7 @@ __global__ __launch_bounds__(block_threads<T>()) void join_bwd_kernel(
 
         float u[NV][N], hat[NV][N], rstd = 1.f;
 #pragma unroll
-        for (int v = 0; v < NV; ++v) unpack_vec<TR>(ro[v], u[v]);
+        for (int v = 0; v < NV; ++v) lane.unpack(ro[v], v, there, u[v]);
         if (p.post_scale) {
             float mean, b[NV][N];
             row_stats<T>(lane, u, p, lds, turn, mean, rstd);
@@ -412,7 +436,7 @@ __global__ __launch_bounds__(block_threads<T>()) void join_bwd_kernel(
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
                 float g[N], dg[N];
-                if (a.gate) unpack_vec<TR>(rg[v], g);
+                if (a.gate) lane.unpack(rg[v], v, there, g);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     const float sig = a.gate ? sigmoid(g[i]) : 1.f;

@@ -14,20 +14,46 @@ struct Vec {
     static constexpr int N = 16 / sizeof(typename TR::elem);
 };
 
-// The N elements from `col` on, zero past the row's end. NT: non-temporal where a vector is aligned
-// (rows that are read once).
+// A row's partial last vector is loaded where the row still holds a whole one and moved down by the
+// difference: a branch to single elements would wait for its loads before the next load is issued.
+
+// The vector without its first s elements of 2 (4) bytes, zeros behind.
+__device__ __forceinline__ u32x4 move_down2(u32x4 r, int s) {
+    r = s & 4 ? u32x4{r[2], r[3], 0u, 0u} : r;
+    r = s & 2 ? u32x4{r[1], r[2], r[3], 0u} : r;
+    return s & 1 ? u32x4{r[0] >> 16 | r[1] << 16, r[1] >> 16 | r[2] << 16, r[2] >> 16 | r[3] << 16,
+                         r[3] >> 16}
+                 : r;
+}
+__device__ __forceinline__ u32x4 move_down4(u32x4 r, int s) {
+    r = s & 2 ? u32x4{r[2], r[3], 0u, 0u} : r;
+    return s & 1 ? u32x4{r[1], r[2], r[3], 0u} : r;
+}
+
+// Moves a vector that was loaded at `at` to `col`, up to N elements on: zeros past the row's end.
+template <typename TR>
+__device__ __forceinline__ u32x4 move_to(u32x4 raw, int at, int col) {
+    return Vec<TR>::N == 8 ? move_down2(raw, col - at) : move_down4(raw, col - at);
+}
+
+// The N elements from `col` < C on, zero past the row's end. NT: non-temporal where a vector is
+// aligned (rows that are read once).
 template <typename TR, bool WHOLE, bool NT = false>
 __device__ __forceinline__ u32x4 load_vec(const typename TR::elem* row, int col, int C) {
     constexpr int N = Vec<TR>::N;
     if (WHOLE && NT) return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(row + col));
     if (WHOLE) return ld16(row + col);
-    if (col + N <= C) return ld16_a2(row + col);
-    typename TR::elem e[N];
+    if (C < N) {  // the same for all rows
+        typename TR::elem e[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) e[i] = col + i < C ? row[col + i] : TR::from_f(0.f);
-    u32x4 raw;
-    __builtin_memcpy(&raw, e, 16);
-    return raw;
+        for (int i = 0; i < N; ++i) e[i] = col + i < C ? row[col + i] : TR::from_f(0.f);
+        u32x4 raw;
+        __builtin_memcpy(&raw, e, 16);
+        return raw;
+    }
+    const int at = col < C - N ? col : C - N;
+    const u32x4 raw = ld16_a2(row + at);
+    return move_to<TR>(raw, at, col);
 }
 
 template <typename TR>
@@ -73,10 +99,13 @@ __device__ __forceinline__ void load_floats(const float* p, int col, int C, floa
                                             float (&out)[N]) {
 #pragma unroll
     for (int q = 0; q < N; q += 4) {
-        if (WHOLE || col + q + 4 <= C) {
-            const f32x4 v = ld4f(p + col + q);
+        if (WHOLE || C >= 4) {
+            const int at = WHOLE || col + q < C - 4 ? col + q : C - 4;
+            u32x4 raw = __builtin_bit_cast(u32x4, ld4f(p + at));
+            if (!WHOLE) raw = move_down4(raw, col + q - at < 4 ? col + q - at : 3);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) out[q + i] = v[i];
+            for (int i = 0; i < 4; ++i)
+                out[q + i] = WHOLE || col + q + i < C ? __uint_as_float(raw[i]) : fill;
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) out[q + i] = col + q + i < C ? p[col + q + i] : fill;
