@@ -997,6 +997,9 @@ extern "C" clk_status clk_embedding_fwd(hipStream_t stream, clk_dtype dtype, con
         return fail(CLK_INVALID_ARGUMENT, "%s: null pointer", who);
     if (!aligned16(table) || !aligned16(out))
         return fail(CLK_INVALID_ARGUMENT, "%s: table and out must be 16-byte aligned", who);
+    const size_t elem = dtype == CLK_F32 ? 4 : 2, id = ids_dtype == CLK_S64 ? 8 : 4;
+    if (overlap(out, M * C * elem, table, V * C * elem) || overlap(out, M * C * elem, ids, M * id))
+        return fail(CLK_INVALID_ARGUMENT, "%s: out may not overlap table or ids", who);
     CLK_EMBED_TYPES(dtype, ids_dtype, launch_fwd, stream, table, ids, out, M, V, C, scale);
     return check_launch(who);
 }
@@ -1030,6 +1033,12 @@ extern "C" clk_status clk_embedding_bwd(hipStream_t stream, clk_dtype dtype, con
     if (workspace_bytes < need)
         return fail(CLK_INVALID_ARGUMENT, "%s: workspace %zu bytes, needs %zu", who,
                     workspace_bytes, need);
+    const size_t in = M * C * (dtype == CLK_F32 ? 4 : 2), id = M * (ids_dtype == CLK_S64 ? 8 : 4);
+    if (overlap(dtable, V * C * 4, dout, in) || overlap(dtable, V * C * 4, ids, id) ||
+        overlap(workspace, need, dout, in) || overlap(workspace, need, ids, id) ||
+        overlap(workspace, need, dtable, V * C * 4))
+        return fail(CLK_INVALID_ARGUMENT, "%s: dout, ids, dtable and workspace may not overlap",
+                    who);
     CLK_EMBED_TYPES(dtype, ids_dtype, launch_bwd, stream, dout, ids, dtable,
                     static_cast<char*>(workspace), M, V, C, scale);
     return check_launch(who);

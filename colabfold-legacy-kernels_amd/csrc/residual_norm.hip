@@ -743,6 +743,20 @@ clk_status validate(const char* who, clk_dtype dtype, int64_t M, int64_t C) {
     return CLK_OK;
 }
 
+// Results may not lie over operands or each other: rows are written while others are read.
+template <size_t NIN, size_t NOUT>
+bool rows_overlap(const void* const (&in)[NIN], const void* const (&out)[NOUT], clk_dtype dtype,
+                  int64_t M, int64_t C) {
+    const size_t bytes = (size_t)M * C * (dtype == CLK_F32 ? 4 : 2);
+    for (size_t i = 0; i < NOUT; ++i) {
+        for (const void* p : in)
+            if (overlap(out[i], bytes, p, bytes)) return true;
+        for (size_t j = 0; j < i; ++j)
+            if (overlap(out[i], bytes, out[j], bytes)) return true;
+    }
+    return false;
+}
+
 clk_status validate_norms(const char* who, clk_norm norm, const float* post_scale,
                           const float* post_offset, const float* pre_scale,
                           const float* pre_offset) {
@@ -775,6 +789,9 @@ extern "C" clk_status clk_residual_norm_fwd(hipStream_t stream, clk_dtype dtype,
     if (!x || !o || !r) return fail(CLK_INVALID_ARGUMENT, "%s: null pointer", who);
     if (!aligned16(x) || !aligned16(o) || !aligned16(gate) || !aligned16(r) || !aligned16(h))
         return fail(CLK_INVALID_ARGUMENT, "%s: x, o, gate, r and h must be 16-byte aligned", who);
+    if (rows_overlap({x, o, gate}, {r, h}, dtype, M, C))
+        return fail(CLK_INVALID_ARGUMENT, "%s: r and h may not overlap x, o, gate or each other",
+                    who);
     const Params p = {post_scale, post_offset, res_scale, pre_scale,
                       pre_offset, M,           (int)C,    norm == CLK_NORM_RMS, eps};
     switch (dtype) {
@@ -825,6 +842,9 @@ extern "C" clk_status clk_residual_norm_bwd(
     if (workspace_bytes < need)
         return fail(CLK_INVALID_ARGUMENT, "%s: workspace %zu bytes, needs %zu", who,
                     workspace_bytes, need);
+    if (rows_overlap({r, o, gate, dr, dh}, {dx, d_o, dgate}, dtype, M, C))
+        return fail(CLK_INVALID_ARGUMENT,
+                    "%s: dx, d_o and dgate may not overlap the operands or each other", who);
     const Params p = {post_scale, post_offset, res_scale, pre_scale,
                       nullptr,    M,           (int)C,    norm == CLK_NORM_RMS, eps};
     float* part = static_cast<float*>(workspace);

@@ -127,6 +127,12 @@ __device__ __forceinline__ void store_floats(float* p, int col, int C, const flo
     }
 }
 
+// Do two arrays of a and b bytes overlap? Null pointers overlap nothing.
+inline bool overlap(const void* p, size_t a, const void* q, size_t b) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(p), y = reinterpret_cast<uintptr_t>(q);
+    return x && y && (x < y ? y - x < a : x - y < b);
+}
+
 inline int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 }  // namespace clk

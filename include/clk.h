@@ -336,7 +336,7 @@ clk_status clk_triangle_multiply(hipStream_t stream, clk_dtype dtype, const void
  * representations begin from): out[i] = scale * table[ids[i]]. An id outside [0, V) is an absent
  * token: its row of out is zero. table and out of dtype CLK_F16, CLK_BF16 or CLK_F32, 16-byte
  * aligned; ids of ids_dtype CLK_S32 or CLK_S64. Any C up to 2^20; M up to 2^30, V below 2^30,
- * M*C and V*C up to 2^37.
+ * M*C and V*C up to 2^37. out may not overlap table or ids.
  */
 clk_status clk_embedding_fwd(hipStream_t stream, clk_dtype dtype, const void* table,
                              clk_dtype ids_dtype, const void* ids, void* out, int64_t M,
@@ -344,9 +344,10 @@ clk_status clk_embedding_fwd(hipStream_t stream, clk_dtype dtype, const void* ta
 
 /*
  * Its backward: dtable[v] = scale * sum of dout[i] over the tokens with ids[i] = v, float32 [V,C];
- * rows that no token names are zero, absent tokens add nothing. Deterministic: the tokens are
- * sorted by row (stably) and summed in a fixed order, no floating-point atomics. dout, dtable and
- * workspace 16-byte aligned; workspace: clk_embedding_bwd_workspace_size bytes.
+ * rows that no token names are zero, absent tokens add nothing. Deterministic: the sums are taken
+ * in a fixed order, no floating-point atomics. dout, dtable and workspace 16-byte aligned; dtable
+ * and workspace may not overlap the other arrays. Workspace: clk_embedding_bwd_workspace_size
+ * bytes.
  */
 size_t clk_embedding_bwd_workspace_size(int64_t M, int64_t V, int64_t C);
 clk_status clk_embedding_bwd(hipStream_t stream, clk_dtype dtype, const void* dout,
@@ -362,7 +363,8 @@ clk_status clk_embedding_bwd(hipStream_t stream, clk_dtype dtype, const void* do
  * N is a LayerNorm (CLK_NORM_LAYER) or an RMS norm (CLK_NORM_RMS, no mean) over the last axis with
  * float32 scale [C] and, where given, offset [C]. post_scale NULL: no norm after the block (u = o);
  * gate NULL: t = u; res_scale NULL: 1; pre_scale NULL: no norm before the next block, and h must be
- * NULL. x, o, gate, r, h of dtype CLK_F16, CLK_BF16 or CLK_F32, 16-byte aligned.
+ * NULL. x, o, gate, r, h of dtype CLK_F16, CLK_BF16 or CLK_F32, 16-byte aligned; r and h may not
+ * overlap the operands or each other.
  */
 clk_status clk_residual_norm_fwd(hipStream_t stream, clk_dtype dtype, clk_norm norm,
                                  const void* x, const void* o, const void* gate,
@@ -377,7 +379,8 @@ clk_status clk_residual_norm_fwd(hipStream_t stream, clk_dtype dtype, clk_norm n
  * Writes dx, d_o and, with gate, dgate [M,C] in the dtype and the column sums dpost_scale,
  * dpost_offset, dres_scale, dpre_scale, dpre_offset [C] float32 (each may be NULL; none for a
  * parameter that is not there). Deterministic. Workspace: clk_residual_norm_bwd_workspace_size
- * bytes, 16-byte aligned. M = 0 writes zero column sums.
+ * bytes, 16-byte aligned. M = 0 writes zero column sums. dx, d_o and dgate may not overlap the
+ * operands or each other.
  */
 size_t clk_residual_norm_bwd_workspace_size(int64_t M, int64_t C);
 clk_status clk_residual_norm_bwd(hipStream_t stream, clk_dtype dtype, clk_norm norm,

@@ -123,6 +123,51 @@ def test_residual_norm_bwd_refuses(kw, msg):
     assert msg in _native.last_error()
 
 
+def spread(names, step=1 << 20):
+    """Addresses far apart for the named arrays."""
+    return {n: FAKE + (i + 1) * step for i, n in enumerate(names)}
+
+
+@pytest.mark.parametrize("first,second,off", [("out", "table", 0), ("out", "table", 240),
+                                              ("table", "out", 112), ("out", "ids", 0),
+                                              ("ids", "out", 124)])
+def test_embedding_refuses_overlaps(first, second, off):
+    at = spread(("table", "ids", "out"))  # out has 4 rows of 32 bytes, the table 8
+    at[first] = at[second] + off
+    assert embedding(**at) == INVALID
+    assert "overlap" in _native.last_error()
+
+
+@pytest.mark.parametrize("first,second,off", [("dtable", "dout", 0), ("dtable", "dout", 112),
+                                              ("dout", "dtable", 496), ("ids", "dtable", 504),
+                                              ("workspace", "dout", 112), ("workspace", "ids", 16),
+                                              ("workspace", "dtable", 496)])
+def test_embedding_bwd_refuses_overlaps(first, second, off):
+    at = spread(("dout", "ids", "dtable", "workspace"))
+    at[first] = at[second] + off
+    assert embedding_bwd(**at) == INVALID
+    assert "overlap" in _native.last_error()
+
+
+@pytest.mark.parametrize("first,second,off", [("r", "x", 0), ("r", "o", 112), ("o", "r", 112),
+                                              ("h", "gate", 16), ("h", "r", 0), ("r", "h", 112)])
+def test_residual_norm_refuses_overlaps(first, second, off):
+    at = spread(("x", "o", "gate", "r", "h"))
+    at[first] = at[second] + off
+    assert residual(**at) == INVALID
+    assert "overlap" in _native.last_error()
+
+
+@pytest.mark.parametrize("first,second,off", [("dx", "dr", 0), ("dx", "r", 112), ("d_o", "o", 0),
+                                              ("dgate", "gate", 0), ("dh", "dx", 16),
+                                              ("dx", "d_o", 0), ("dgate", "dx", 112)])
+def test_residual_norm_bwd_refuses_overlaps(first, second, off):
+    at = spread(("r", "o", "gate", "dr", "dh", "dx", "d_o", "dgate"))
+    at[first] = at[second] + off
+    assert residual_bwd(**at) == INVALID
+    assert "overlap" in _native.last_error()
+
+
 def test_ops_refuse_host_tensors():
     t = torch.zeros(4, 8)
     for call in (lambda: ops.embedding(t, torch.zeros(3, dtype=torch.long)),
