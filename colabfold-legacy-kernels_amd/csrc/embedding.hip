@@ -4,9 +4,14 @@
 //   dtable[v] = scale * sum of dout[i] over ids[i] = v      absent token: a zero row, no gradient
 //
 // The forward is one pass that writes M*C*b bytes (the rows of a table that is used often stay in
-// the L2s). The gradient sorts the tokens by row (stably, so that the order of every sum is fixed),
-// sums runs of equal rows over the sorted order and joins the runs that were cut; it reads dout
-// once, in whole rows of at least 256 bytes where a row has them, and writes the table once.
+// the L2s): 262144 tokens of 128 bf16 columns in 11.8 us, 5.7 TB/s.
+//
+// The gradient of a table of few rows is a product on the matrix cores that reads dout once, in
+// order (147456 tokens, 65 rows of 128 bf16 columns: 17 us, of which the bytes need 7; sorting took
+// 76). Others sort the tokens by row (stably, so that the order of every sum is fixed), sum runs of
+// equal rows over the sorted order and join the runs that were cut; dout is read once, in whole
+// rows of at least 256 bytes where a row has them (16411 tokens, 30011 rows of 640 float16 columns:
+// 44 us, of which the bytes need 17 and the sort's four launches, with the zeros they write, 27).
 #include "rows.hpp"
 
 namespace clk {
