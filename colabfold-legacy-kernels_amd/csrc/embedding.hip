@@ -543,10 +543,34 @@ __device__ __forceinline__ Four<TR> load_four(const typename TR::elem* row, int 
 
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 
+// The A operand of 16 rows: 1 - |id ^ row|, saturated at 0, is whether they are equal; times the
+// bits of 1.
+template <typename TR>
+__device__ __forceinline__ typename TR::vec8 onehot(const u16x2 (&ids)[4], unsigned short row) {
+    const unsigned short one = (unsigned short)kOnePair<TR>;
+    u16x2 a[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        a[q] = __builtin_elementwise_sub_sat(u16x2{1, 1}, ids[q] ^ u16x2{row, row}) *
+               u16x2{one, one};
+    typename TR::vec8 av;
+    __builtin_memcpy(&av, a, 16);
+    return av;
+}
+
 // One step of 32 tokens: acc[v][ct] += onehot . columns.
+//
+// A float32 column is the sum of three bf16 ones, its bits cut after 8, 16 and 24 (exactly, but for
+// what lies below 2^-133), and three products of bf16 take a fifth of the matrix cores' time of one
+// of float32: 147456 tokens of 65 rows of 128 columns 22 us instead of 36, 131072 of 23 rows of 256
+// columns 30.4 instead of 33.4 (24 by their bytes).
 template <typename TR, int VT>
 __device__ __forceinline__ void hot_step(const int (&id)[8], const Four<TR> (&x)[8], int r16,
                                          f32x4 (&acc)[VT][4]) {
+    u16x2 ids[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        ids[q] = u16x2{(unsigned short)id[2 * q], (unsigned short)id[2 * q + 1]};
     if constexpr (sizeof(typename TR::elem) == 2) {
         using V8 = typename TR::vec8;
         V8 b[4];
@@ -554,36 +578,42 @@ __device__ __forceinline__ void hot_step(const int (&id)[8], const Four<TR> (&x)
         for (int ct = 0; ct < 4; ++ct)
 #pragma unroll
             for (int j = 0; j < 8; ++j) b[ct][j] = x[j].e[ct];
-        u16x2 ids[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-            ids[q] = u16x2{(unsigned short)id[2 * q], (unsigned short)id[2 * q + 1]};
-        const unsigned short one = (unsigned short)kOnePair<TR>;
 #pragma unroll
         for (int v = 0; v < VT; ++v) {
-            // 1 - |id ^ row|, saturated at 0, is whether they are equal; times the bits of 1.
-            const unsigned short row = (unsigned short)(16 * v + r16);
-            u16x2 a[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-                a[q] = __builtin_elementwise_sub_sat(u16x2{1, 1}, ids[q] ^ u16x2{row, row}) *
-                       u16x2{one, one};
-            V8 av;
-            __builtin_memcpy(&av, a, 16);
+            const V8 av = onehot<TR>(ids, (unsigned short)(16 * v + r16));
 #pragma unroll
             for (int ct = 0; ct < 4; ++ct) acc[v][ct] = TR::mfma(av, b[ct], acc[v][ct]);
         }
     } else {
+        using V8 = BF16::vec8;
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
+        for (int ct = 0; ct < 4; ++ct) {
+            // Many rows' A operands are made again for each column: kept, they would spill.
+            if constexpr (VT > 5)
+                asm volatile("" : "+v"(ids[0]), "+v"(ids[1]), "+v"(ids[2]), "+v"(ids[3]));
+            uint32_t w[3][4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                float f0 = x[2 * q].e[ct], f1 = x[2 * q + 1].e[ct];
+#pragma unroll
+                for (int k = 0; k < 3; ++k) {
+                    const uint32_t u0 = __float_as_uint(f0), u1 = __float_as_uint(f1);
+                    w[k][q] = __builtin_amdgcn_perm(u1, u0, 0x07060302u);
+                    f0 -= __uint_as_float(u0 & 0xFFFF0000u);
+                    f1 -= __uint_as_float(u1 & 0xFFFF0000u);
+                }
+            }
+            V8 b[3];
+            __builtin_memcpy(&b, w, sizeof(w));
 #pragma unroll
             for (int v = 0; v < VT; ++v) {
-                const float a = id[j] == 16 * v + r16 ? 1.f : 0.f;
+                const V8 av = onehot<BF16>(ids, (unsigned short)(16 * v + r16));
 #pragma unroll
-                for (int ct = 0; ct < 4; ++ct)
-                    acc[v][ct] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, x[j].e[ct], acc[v][ct], 0,
-                                                                      0, 0);
+                for (int k = 2; k >= 0; --k)  // the smallest first
+                    acc[v][ct] = BF16::mfma(av, b[k], acc[v][ct]);
             }
+            __builtin_amdgcn_sched_barrier(0);  // one column's operands at a time
+        }
     }
 }
 
@@ -634,7 +664,8 @@ __global__ __launch_bounds__(64 * kHotWaves) void embed_hot_kernel(
         }
     };
     constexpr int64_t kNext = WT * kStep;
-    if constexpr (VT <= 5) {  // two steps in flight
+    // Two steps in flight where there are registers for them.
+    if constexpr (VT <= 2 || (VT <= 5 && (WHOLE || sizeof(typename TR::elem) == 2))) {
         int id0[8], id1[8];
         Four<TR> x0[8], x1[8];
         if (first < end) load(first, id0, x0);
@@ -646,7 +677,7 @@ __global__ __launch_bounds__(64 * kHotWaves) void embed_hot_kernel(
                 hot_step<TR, VT>(id1, x1, r16, acc);
             }
         }
-    } else {  // no registers for a second one
+    } else {
         for (int64_t t0 = first; t0 < end; t0 += kNext) {
             int id[8];
             Four<TR> x[8];
@@ -782,13 +813,14 @@ BwdPlan bwd_plan(int64_t M, int64_t V, int64_t C, bool half) {
     BwdPlan p = {};
     if (hot_table(M, V, C)) {
         // As many blocks as CUs, with at least two steps of tokens a wave; up to eight where one
-        // block can then take all tokens and the partials' kernel is saved (the float32 products
-        // of eight steps would take longer than it).
+        // block can then take all tokens and the partials' kernel is saved (not where float32 steps
+        // of many rows take longer than it: 900 tokens of 129 rows of 256 columns 17 us in blocks,
+        // 32 in one; 700 of 30 rows of 100 columns 13.5 and 11).
         p.hot = true;
         const int64_t others = up(C, C > kHotCols ? 2 * kHotCols : kHotCols) * up(V, kHotRows);
         const int64_t want = std::max<int64_t>(1, 256 / others);
         const int64_t round = kStep * (C > kHotCols ? kHotWaves / 2 : kHotWaves);
-        const int64_t least = half && M <= 8 * round ? M : 2 * round;
+        const int64_t least = (half || V <= 32) && M <= 8 * round ? M : 2 * round;
         p.tokens = up(std::max(up(M, want), std::min(M, least)), kStep) * kStep;
         p.parts = (int)up(M, p.tokens);
         p.stride = (size_t)up(V * C, 4) * 4;

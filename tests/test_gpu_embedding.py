@@ -299,3 +299,35 @@ def test_gradient_at_the_borders_of_row_blocks(cuda, dtype, v):
     assert (err <= 2 * (count[ok][:, None] + 3) * U32 * size[ok] + 1e-37).all()
     assert got[0].isnan().all() and got[142, 5] == float("inf")
     assert torch.isfinite(got[142, torch.arange(c, device=cuda) != 5]).all()
+
+
+@pytest.mark.parametrize("dtype,unit", [(torch.float16, 2.0 ** -24), (torch.bfloat16, 2.0 ** -133),
+                                        (torch.float32, 2.0 ** -133)])
+@pytest.mark.parametrize("v", [20, 65, 129, 3000])
+def test_gradient_of_subnormal_numbers(cuda, dtype, unit, v):
+    """Small multiples of a unit below the normal range: every sum of them is exact."""
+    g = torch.Generator().manual_seed(7)
+    dout = (torch.randint(-3, 4, (640, 43), generator=g).double() * unit).to(dtype).to(cuda)
+    ids = torch.randint(0, v, (640,), generator=g).to(cuda)
+    got = ops.embedding_bwd(dout, ids, v)
+    want = ref.embedding_bwd(np64(dout), ids.cpu().numpy(), v, 1.0)
+    assert np.array_equal(np64(got), want)
+
+
+@pytest.mark.parametrize("m,v,c", [(1, 1, 5), (700, 30, 100), (5000, 65, 131), (5000, 65, 128),
+                                   (900, 129, 256), (4000, 144, 77), (2500, 300, 64)])
+def test_float32_gradient_of_single_tokens_is_exact(cuda, m, v, c):
+    """A row that one token names is that token's row, to the last bit, at every size from the
+    smallest normal number that holds 24 bits above 2^-133 to the largest finite one."""
+    g = torch.Generator().manual_seed(11)
+    ids = torch.randint(0, max(v // 2, 1), (m,), generator=g)
+    alone = torch.arange(max(v // 2, 1), v)[:m]  # rows of one token each
+    at = torch.randperm(m, generator=g)[:alone.numel()]
+    ids[at] = alone
+    x = torch.randn(m, c, generator=g)
+    x[at] = torch.randn(alone.numel(), c, generator=g) * 2.0 ** torch.randint(
+        -100, 120, (alone.numel(), 1), generator=g).float()
+    if m > 1:
+        x[at[0], 0] = torch.finfo(torch.float32).max
+    got = ops.embedding_bwd(x.to(cuda), ids.to(cuda), v).cpu()
+    assert torch.equal(got[ids[at]], x[at])
